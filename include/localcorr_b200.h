@@ -21,7 +21,8 @@
  * false for an invalid configuration or a launch error; the reason is then
  * available from localCorrB200GetLastError() (thread-local).
  *
- * dtype codes: LCB200_F32 = 0 (float32), LCB200_F16 = 1 (float16).
+ * dtype codes: LCB200_F32 = 0 (float32), LCB200_F16 = 1 (float16),
+ * LCB200_BF16 = 2 (bfloat16, the feature-map operators only).
  */
 #ifndef LOCALCORR_B200_H
 #define LOCALCORR_B200_H
@@ -42,6 +43,7 @@ extern "C" {
 
 #define LCB200_F32 0
 #define LCB200_F16 1
+#define LCB200_BF16 2
 
 /* Engine selection for the extended pyramid launchers. */
 #define LCB200_ENGINE_AUTO 0    /* tensor-core engine when eligible, else CUDA-core */
@@ -289,6 +291,63 @@ LCB200_API bool launchLocalCorrB200PyramidBackwardFmap2Pull(
     const void* const* sort_states, const void* const* records, int nlookups,
     float* fmap2_grad_f32, int B, int H1, int W1, int H2, int W2, int C, int radius, int levels,
     float scale, int accumulate, void* workspace, size_t workspace_bytes, cudaStream_t stream);
+
+/* ---- Feature-map operators ---------------------------------------------------
+ * No reference counterpart (the reference leaves the encoder to torch). The
+ * maps are channels last, [B, rows, C] contiguous, rows the product of the
+ * spatial sizes; dtype float32, float16 or bfloat16. Results are rounded to
+ * dtype once. No float atomics: equal inputs give equal bits.
+ *
+ * Dropout draws: Philox4x32-10 with key seed and counter (block, offset);
+ * draw e is 16-bit piece e % 8 (low half of a word first) of block e / 8, and
+ * drops when it is below round(65536 p); what stays is multiplied by
+ * 65536 / (65536 - round(65536 p)), what drops becomes 0 whatever it held.
+ * e is the element's index in [B, rows, C], or b*C + c with channel = true
+ * (whole channels of a sample). The stream (seed, offset) is the two
+ * long longs at `rng` (device; a captured graph can advance them between
+ * replays) or, with rng NULL, the arguments seed and offset. rng_used (device,
+ * two long longs, may be NULL) receives the stream that was used; pass it as
+ * `rng` of the backward. */
+
+/* y = residual + dropout(x); residual may be NULL. The gradient of x is the
+ * same call on the output gradient without a residual (the residual's
+ * gradient is the output gradient). x, residual and y do not overlap. */
+LCB200_API bool launchLocalCorrB200Dropout(const void* x, const void* residual, void* y, int B,
+                                           long long rows, int C, int dtype, double p,
+                                           bool channel, long long seed, long long offset,
+                                           const long long* rng, long long* rng_used,
+                                           cudaStream_t stream);
+
+/* Activations behind the group norm. */
+#define LCB200_ACT_NONE 0
+#define LCB200_ACT_RELU 1
+#define LCB200_ACT_SILU 2
+#define LCB200_ACT_LEAKY_RELU 3
+
+/* y = dropout(act(group_norm(x))): per sample and group of C/groups
+ * consecutive channels, (x - mean) / sqrt(var + eps) * weight + bias (biased
+ * variance over rows and the group's channels), the activation (negative_slope
+ * is LEAKY_RELU's), and with p > 0 dropout. weight and bias: [C], either may
+ * be NULL (1 and 0), of float32 (param_f32) or of dtype. stats receives
+ * [B, groups] pairs of float64 (mean, 1/sqrt(var + eps)), 16-byte aligned. */
+LCB200_API size_t localCorrB200GroupNormWorkspaceBytes(int B, long long rows, int C, int groups,
+                                                       int dtype, bool backward);
+LCB200_API bool launchLocalCorrB200GroupNormForward(
+    const void* x, const void* weight, const void* bias, void* y, double* stats, int B,
+    long long rows, int C, int groups, int dtype, bool param_f32, double eps, int activation,
+    float negative_slope, double p, bool channel, long long seed, long long offset,
+    const long long* rng, long long* rng_used, void* workspace, size_t workspace_bytes,
+    cudaStream_t stream);
+
+/* Gradients for the same arguments; stats from the forward, and with p > 0
+ * its stream. grad_x like x; grad_weight / grad_bias like weight / bias;
+ * what is NULL is not computed. */
+LCB200_API bool launchLocalCorrB200GroupNormBackward(
+    const void* grad_y, const void* x, const void* weight, const void* bias, const double* stats,
+    void* grad_x, void* grad_weight, void* grad_bias, int B, long long rows, int C, int groups,
+    int dtype, bool param_f32, int activation, float negative_slope, double p, bool channel,
+    long long seed, long long offset, const long long* rng, void* workspace,
+    size_t workspace_bytes, cudaStream_t stream);
 
 /* ---- Deterministic mode ---------------------------------------------------
  * No reference counterpart (the reference's backward adds grad_fmap2 with

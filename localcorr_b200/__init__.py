@@ -28,6 +28,7 @@ from .blocks import (
 )
 from .blocks import LocalCorrCudaPyramidSpatialOnnx
 from .spatial_corr import LocalCorrCudaPyramidSampler, get_sycl_xpu_extension
+from .features import dropout, group_norm
 from .ops import is_deterministic, set_deterministic
 
 # The reference's Triton autograd Functions (triton/pyramid_corr.py:845-1246,
@@ -66,4 +67,6 @@ __all__ = [
     "TritonSpatialCorrelationSampler",
     "set_deterministic",
     "is_deterministic",
+    "group_norm",
+    "dropout",
 ]

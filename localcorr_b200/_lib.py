@@ -25,8 +25,10 @@ LIB_PATH = LIB_PATH_CHECKED if BOUNDS_CHECK else LIB_PATH_DEFAULT
 
 F32 = 0
 F16 = 1
+BF16 = 2  # feature-map operators only
 ACC_FMAP2 = 1  # backward: add into the float32 fmap2 gradient
 ACC_FMAP1 = 2  # backward: add into the fmap1 gradient
+ACT_CODES = {"none": 0, "relu": 1, "silu": 2, "leaky_relu": 3}
 ENGINE_AUTO = 0
 ENGINE_SIMT = 1
 ENGINE_TC = 2
@@ -36,6 +38,8 @@ _c_int = ctypes.c_int
 _c_bool = ctypes.c_bool
 _c_float = ctypes.c_float
 _c_size_t = ctypes.c_size_t
+_c_double = ctypes.c_double
+_c_longlong = ctypes.c_longlong
 
 # name -> (restype, argtypes). Every exported symbol of include/localcorr_b200.h.
 PROTOTYPES = {
@@ -120,6 +124,25 @@ PROTOTYPES = {
         _c_bool,
         [ctypes.POINTER(_c_void_p)] * 2 + [_c_int, _c_void_p] + [_c_int] * 8
         + [_c_float, _c_int, _c_void_p, _c_size_t, _c_void_p],
+    ),
+    "launchLocalCorrB200Dropout": (
+        _c_bool,
+        [_c_void_p] * 3 + [_c_int, _c_longlong, _c_int, _c_int, _c_double, _c_bool, _c_longlong,
+                           _c_longlong, _c_void_p, _c_void_p, _c_void_p],
+    ),
+    "localCorrB200GroupNormWorkspaceBytes": (
+        _c_size_t, [_c_int, _c_longlong, _c_int, _c_int, _c_int, _c_bool]),
+    "launchLocalCorrB200GroupNormForward": (
+        _c_bool,
+        [_c_void_p] * 5 + [_c_int, _c_longlong, _c_int, _c_int, _c_int, _c_bool, _c_double,
+                           _c_int, _c_float, _c_double, _c_bool, _c_longlong, _c_longlong,
+                           _c_void_p, _c_void_p, _c_void_p, _c_size_t, _c_void_p],
+    ),
+    "launchLocalCorrB200GroupNormBackward": (
+        _c_bool,
+        [_c_void_p] * 8 + [_c_int, _c_longlong, _c_int, _c_int, _c_int, _c_bool, _c_int,
+                           _c_float, _c_double, _c_bool, _c_longlong, _c_longlong, _c_void_p,
+                           _c_void_p, _c_size_t, _c_void_p],
     ),
     "localCorrB200GetLastError": (ctypes.c_char_p, []),
     "localCorrB200DeviceStatus": (_c_int, [_c_int]),

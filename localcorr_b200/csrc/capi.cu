@@ -5,10 +5,11 @@
 
 #include <algorithm>
 #include <atomic>
+#include <initializer_list>
 #include <mutex>
 #include <string>
 
-#include "lc_common.cuh"
+#include "feature_common.cuh"
 
 namespace lcb200 {
 
@@ -56,6 +57,14 @@ bool layout_nhwc_to_nchw(const void*, void*, int, int, int, int, cudaStream_t);
 bool layout_pyramid_build(const void*, void*, int, int, int, int, int, int, cudaStream_t);
 bool layout_pyramid_build_grad(const void*, bool, void*, int, int, int, int, int, int,
                                cudaStream_t);
+bool feature_dropout(const void* x, const void* residual, void* y, int B, long long rows, int C,
+                     int dtype, const DropArgs& d, cudaStream_t s);
+size_t feature_norm_workspace(int B, long long S, int C, int G, int dtype, bool backward);
+bool feature_norm(const void* x, const void* dy, const void* weight, const void* bias, void* out,
+                  double* stats, void* dweight, void* dbias, int B, long long S, int C, int G,
+                  int dtype, bool param_f32, double eps, int act, float slope,
+                  const DropArgs& drop, void* ws, size_t ws_bytes, bool backward,
+                  cudaStream_t s);
 bool spatial_forward(const void*, const void*, void*, int, int, int, int, int, int, int, float,
                      cudaStream_t);
 bool spatial_backward(const void*, const void*, const void*, void*, void*, int, int, int, int,
@@ -158,6 +167,24 @@ int max_dyn_smem() {
   int v = 0;
   if (cudaDeviceGetAttribute(&v, cudaDevAttrMaxSharedMemoryPerBlockOptin, dev) != cudaSuccess)
     v = 48 * 1024;
+  return v;
+}
+
+int device_sms() {
+  static std::atomic<int> table[64];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) {
+    cudaGetLastError();
+    return 148;
+  }
+  int v = table[dev].load(std::memory_order_relaxed);
+  if (v == 0) {
+    if (cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || v < 1) {
+      cudaGetLastError();
+      v = 148;
+    }
+    table[dev].store(v, std::memory_order_relaxed);
+  }
   return v;
 }
 
@@ -502,6 +529,69 @@ bool validate_layout(int B, int C, int H, int W, int dtype) {
   return true;
 }
 
+// Shapes, dtype and dropout arguments of the feature-map operators.
+bool validate_feature(int B, long long rows, int C, int dtype, bool* empty) {
+  *empty = false;
+  if (dtype != LCB200_F32 && dtype != LCB200_F16 && dtype != LCB200_BF16) {
+    set_error("dtype must be LCB200_F32 (0), LCB200_F16 (1) or LCB200_BF16 (2)");
+    return false;
+  }
+  if (B < 0 || rows < 0 || C < 1) {
+    set_error("invalid shape: B=" + std::to_string(B) + ", rows=" + std::to_string(rows) +
+              ", C=" + std::to_string(C));
+    return false;
+  }
+  if ((double)B * (double)rows * (double)C > 1e18) {
+    set_error("too many elements");
+    return false;
+  }
+  *empty = B == 0 || rows == 0;
+  return true;
+}
+
+bool make_drop(double p, bool channel, long long seed, long long offset, const long long* rng,
+               long long* rng_used, DropArgs* d) {
+  if (!(p >= 0.0 && p <= 1.0)) {  // NaN fails too
+    set_error("dropout probability must be in [0, 1]");
+    return false;
+  }
+  d->threshold = (uint32_t)(p * 65536.0 + 0.5);
+  d->factor = d->threshold >= 65536u ? 0.f : (float)(65536.0 / (65536u - d->threshold));
+  d->channel = channel;
+  d->seed = seed;
+  d->offset = offset;
+  d->rng = rng;
+  d->rng_used = rng_used;
+  return true;
+}
+
+// Every pointer a multiple of `align` (null is).
+bool aligned(size_t align, std::initializer_list<const void*> ptrs, const char* what) {
+  for (const void* p : ptrs)
+    if (reinterpret_cast<uintptr_t>(p) % align) {
+      set_error(std::string(what) + " must be " + std::to_string(align) + "-byte aligned");
+      return false;
+    }
+  return true;
+}
+
+bool validate_norm(int groups, int C, int activation, float slope) {
+  if (groups < 1 || C % groups != 0) {
+    set_error("groups must divide C (C=" + std::to_string(C) + ", groups=" +
+              std::to_string(groups) + ")");
+    return false;
+  }
+  if (activation < LCB200_ACT_NONE || activation > LCB200_ACT_LEAKY_RELU) {
+    set_error("unknown activation " + std::to_string(activation));
+    return false;
+  }
+  if (!(slope - slope == 0.f)) {
+    set_error("negative_slope must be finite");
+    return false;
+  }
+  return true;
+}
+
 }  // namespace
 }  // namespace lcb200
 
@@ -787,6 +877,102 @@ bool launchLocalCorrB200SpatialBackward(const void* in1, const void* in2, const 
       spatial_backward(in1, in2, grad_out, grad_in1, grad_in2, B, C, H, W, radius, dilation,
                           dtype, scale, stream),
       stream);
+}
+
+bool launchLocalCorrB200Dropout(const void* x, const void* residual, void* y, int B,
+                                long long rows, int C, int dtype, double p, bool channel,
+                                long long seed, long long offset, const long long* rng,
+                                long long* rng_used, cudaStream_t stream) {
+  clear_error();
+  bool empty = false;
+  DropArgs d{};
+  if (!validate_feature(B, rows, C, dtype, &empty) ||
+      !make_drop(p, channel, seed, offset, rng, rng_used, &d) ||
+      !aligned(dtype_bytes(dtype), {x, residual, y}, "dropout: maps") ||
+      !aligned(8, {rng, rng_used}, "dropout: rng"))
+    return false;
+  if (empty) return true;
+  if (!x || !y) {
+    set_error("dropout: null map");
+    return false;
+  }
+  NvtxRange range("localcorr_b200 dropout");
+  return feature_dropout(x, residual, y, B, rows, C, dtype, d, stream);
+}
+
+size_t localCorrB200GroupNormWorkspaceBytes(int B, long long rows, int C, int groups, int dtype,
+                                            bool backward) {
+  clear_error();
+  bool empty = false;
+  if (!validate_feature(B, rows, C, dtype, &empty) || empty ||
+      !validate_norm(groups, C, LCB200_ACT_NONE, 0.f))
+    return 0;
+  return feature_norm_workspace(B, rows, C, groups, dtype, backward);
+}
+
+bool launchLocalCorrB200GroupNormForward(
+    const void* x, const void* weight, const void* bias, void* y, double* stats, int B,
+    long long rows, int C, int groups, int dtype, bool param_f32, double eps, int activation,
+    float negative_slope, double p, bool channel, long long seed, long long offset,
+    const long long* rng, long long* rng_used, void* workspace, size_t workspace_bytes,
+    cudaStream_t stream) {
+  clear_error();
+  bool empty = false;
+  DropArgs d{};
+  if (!validate_feature(B, rows, C, dtype, &empty) ||
+      !validate_norm(groups, C, activation, negative_slope) ||
+      !make_drop(p, channel, seed, offset, rng, rng_used, &d) ||
+      !aligned(dtype_bytes(dtype), {x, y}, "group norm: maps") ||
+      !aligned(param_f32 ? 4 : dtype_bytes(dtype), {weight, bias}, "group norm: weight and bias") ||
+      !aligned(16, {stats}, "group norm: stats") || !aligned(8, {rng, rng_used}, "group norm: rng"))
+    return false;
+  if (!(eps >= 0.0 && eps <= 1e30)) {
+    set_error("eps must be finite and not negative");
+    return false;
+  }
+  if (empty) return true;
+  if (!x || !y || !stats) {
+    set_error("group norm: null map or stats");
+    return false;
+  }
+  NvtxRange range("localcorr_b200 group norm forward");
+  return feature_norm(x, nullptr, weight, bias, y, stats, nullptr, nullptr, B, rows, C, groups,
+                      dtype, param_f32, eps, activation, negative_slope, d, workspace,
+                      workspace_bytes, false, stream);
+}
+
+bool launchLocalCorrB200GroupNormBackward(
+    const void* grad_y, const void* x, const void* weight, const void* bias, const double* stats,
+    void* grad_x, void* grad_weight, void* grad_bias, int B, long long rows, int C, int groups,
+    int dtype, bool param_f32, int activation, float negative_slope, double p, bool channel,
+    long long seed, long long offset, const long long* rng, void* workspace,
+    size_t workspace_bytes, cudaStream_t stream) {
+  clear_error();
+  bool empty = false;
+  DropArgs d{};
+  if (!validate_feature(B, rows, C, dtype, &empty) ||
+      !validate_norm(groups, C, activation, negative_slope) ||
+      !make_drop(p, channel, seed, offset, rng, nullptr, &d) ||
+      !aligned(dtype_bytes(dtype), {grad_y, x, grad_x}, "group norm: maps") ||
+      !aligned(param_f32 ? 4 : dtype_bytes(dtype), {weight, bias, grad_weight, grad_bias},
+               "group norm: weight and bias") ||
+      !aligned(16, {stats}, "group norm: stats") || !aligned(8, {rng}, "group norm: rng"))
+    return false;
+  if (empty) {  // sums over nothing
+    const size_t bytes = (param_f32 ? 4 : dtype_bytes(dtype)) * (size_t)C;
+    if ((grad_weight && cudaMemsetAsync(grad_weight, 0, bytes, stream) != cudaSuccess) ||
+        (grad_bias && cudaMemsetAsync(grad_bias, 0, bytes, stream) != cudaSuccess))
+      return check_launch("group norm backward: memset");
+    return true;
+  }
+  if (!grad_y || !x || !stats) {
+    set_error("group norm backward: null map or stats");
+    return false;
+  }
+  NvtxRange range("localcorr_b200 group norm backward");
+  return feature_norm(x, grad_y, weight, bias, grad_x, const_cast<double*>(stats), grad_weight,
+                      grad_bias, B, rows, C, groups, dtype, param_f32, 0.0, activation,
+                      negative_slope, d, workspace, workspace_bytes, true, stream);
 }
 
 const char* localCorrB200GetLastError(void) { return g_last_error.c_str(); }

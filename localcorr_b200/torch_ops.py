@@ -23,15 +23,23 @@ Operators (CUDA tensors only; all outputs are new tensors):
   (blocks.py:534-537).
 * ``spatial_corr(in1, in2, radius, dilation, scale)``: [B, RD, RD, H, W] on
   NCHW inputs (radius <= 4). Backward: ``spatial_corr_backward``.
+* ``group_norm(x, weight, bias, num_groups, eps, activation, negative_slope, p,
+  channel, rng, seed, offset)``: (dropout(act(group norm)) of a channels-last
+  map, its statistics, the dropout stream used), see :mod:`localcorr_b200.features`.
+  Backward: ``group_norm_backward``.
+* ``dropout(x, residual, p, channel, rng, seed, offset)``: (residual +
+  dropout(x), the stream used). Backward: ``dropout_backward``.
 """
 
 from __future__ import annotations
+
+from typing import Optional
 
 import torch
 from torch import Tensor
 from torch.library import custom_op
 
-from . import ops
+from . import features, ops
 
 _NS = "localcorr"
 
@@ -225,3 +233,98 @@ def _sc_backward(ctx, g):
 
 
 spatial_corr.register_autograd(_sc_backward, setup_context=_sc_setup)
+
+
+# ---------------------------------------------------------------------------
+# feature-map operators
+# ---------------------------------------------------------------------------
+
+@custom_op(f"{_NS}::group_norm", mutates_args=(), device_types="cuda")
+def group_norm(x: Tensor, weight: Optional[Tensor], bias: Optional[Tensor], num_groups: int,
+               eps: float, activation: str, negative_slope: float, p: float, channel: bool,
+               rng: Optional[Tensor], seed: int, offset: int) -> tuple[Tensor, Tensor, Tensor]:
+    return features.group_norm_forward(x, weight, bias, num_groups, eps, activation,
+                                       negative_slope, p, channel, rng, seed, offset)
+
+
+@group_norm.register_fake
+def _(x, weight, bias, num_groups, eps, activation, negative_slope, p, channel, rng, seed,
+      offset):
+    return (x.new_empty(x.shape), x.new_empty((x.shape[0], num_groups, 2), dtype=torch.float64),
+            x.new_empty((2 if p > 0 else 0,), dtype=torch.int64))
+
+
+def _absent(like: Tensor) -> Tensor:
+    return like.new_empty((0,))
+
+
+@custom_op(f"{_NS}::group_norm_backward", mutates_args=(), device_types="cuda")
+def group_norm_backward(grad_y: Tensor, x: Tensor, weight: Optional[Tensor],
+                        bias: Optional[Tensor], stats: Tensor, used: Tensor, num_groups: int,
+                        activation: str, negative_slope: float, p: float,
+                        channel: bool) -> tuple[Tensor, Tensor, Tensor]:
+    """Gradients of x, weight and bias (empty for an absent parameter)."""
+    gx, gw, gb = features.group_norm_backward(grad_y, x, weight, bias, stats, used, num_groups,
+                                              activation, negative_slope, p, channel)
+    return gx, gw if gw is not None else _absent(x), gb if gb is not None else _absent(x)
+
+
+@group_norm_backward.register_fake
+def _(grad_y, x, weight, bias, stats, used, num_groups, activation, negative_slope, p, channel):
+    return (x.new_empty(x.shape),
+            weight.new_empty(weight.shape) if weight is not None else _absent(x),
+            bias.new_empty(bias.shape) if bias is not None else _absent(x))
+
+
+def _gn_setup(ctx, inputs, output):
+    x, weight, bias, num_groups, _, activation, slope, p, channel, _, _, _ = inputs
+    _, stats, used = output
+    ctx.save_for_backward(x, weight, bias, stats, used)
+    ctx.params = (num_groups, activation, slope, p, channel)
+
+
+def _gn_backward(ctx, gy, _stats, _used):
+    x, weight, bias, stats, used = ctx.saved_tensors
+    gx, gw, gb = torch.ops.localcorr.group_norm_backward(gy, x, weight, bias, stats, used,
+                                                         *ctx.params)
+    return (gx, gw if weight is not None else None, gb if bias is not None else None,
+            *[None] * 9)
+
+
+group_norm.register_autograd(_gn_backward, setup_context=_gn_setup)
+
+
+@custom_op(f"{_NS}::dropout", mutates_args=(), device_types="cuda")
+def dropout(x: Tensor, residual: Optional[Tensor], p: float, channel: bool,
+            rng: Optional[Tensor], seed: int, offset: int) -> tuple[Tensor, Tensor]:
+    return features.dropout_forward(x, residual, p, channel, rng, seed, offset)
+
+
+@dropout.register_fake
+def _(x, residual, p, channel, rng, seed, offset):
+    return x.new_empty(x.shape), x.new_empty((2,), dtype=torch.int64)
+
+
+@custom_op(f"{_NS}::dropout_backward", mutates_args=(), device_types="cuda")
+def dropout_backward(grad_y: Tensor, used: Tensor, p: float, channel: bool) -> Tensor:
+    return features.dropout_backward(grad_y, used, p, channel)
+
+
+@dropout_backward.register_fake
+def _(grad_y, used, p, channel):
+    return grad_y.new_empty(grad_y.shape)
+
+
+def _do_setup(ctx, inputs, output):
+    _, residual, p, channel, _, _, _ = inputs
+    ctx.save_for_backward(output[1])
+    ctx.params = (p, channel)
+    ctx.residual = residual is not None
+
+
+def _do_backward(ctx, gy, _used):
+    gx = torch.ops.localcorr.dropout_backward(gy, ctx.saved_tensors[0], *ctx.params)
+    return (gx, gy if ctx.residual else None, *[None] * 5)
+
+
+dropout.register_autograd(_do_backward, setup_context=_do_setup)
