@@ -52,6 +52,7 @@ bool tc_pull_lookups(const void* const* sort_states, const void* const* records,
 bool tc_bwd_eligible(int B, int H1, int W1, int H2, int W2, int C, int radius, int levels,
                      int dilation, int dtype, std::string* why);
 int tc_device_status(bool reset);
+int feature_device_status(bool reset);
 bool layout_nchw_to_nhwc(const void*, void*, int, int, int, int, cudaStream_t);
 bool layout_nhwc_to_nchw(const void*, void*, int, int, int, int, cudaStream_t);
 bool layout_pyramid_build(const void*, void*, int, int, int, int, int, int, cudaStream_t);
@@ -977,7 +978,9 @@ bool launchLocalCorrB200GroupNormBackward(
 
 const char* localCorrB200GetLastError(void) { return g_last_error.c_str(); }
 
-int localCorrB200DeviceStatus(int reset) { return tc_device_status(reset != 0); }
+int localCorrB200DeviceStatus(int reset) {
+  return tc_device_status(reset != 0) | feature_device_status(reset != 0);
+}
 
 int localCorrB200Version(void) { return 100; }
 

@@ -1,140 +1,15 @@
-// Group normalisation with an activation, channels last: x [B, S, C], groups of
-// Cg = C / G consecutive channels, n = S * Cg values a group.
-//
-//   forward   mu = sum x / n, var = sum (x - mu)^2 / n, r = (var + eps)^-1/2,
-//             z = (x - mu) r gamma + beta, y = drop(act(z))
-//   backward  dz = drop'(dy) act'(z), A = sum_s dz, X = sum_s dz (x - mu) r,
-//             dbeta = sum_b A, dgamma = sum_b X,
-//             m1 = sum_g gamma A / n, m2 = sum_g gamma X / n,
-//             dx = r (gamma dz - m1 - (x - mu) r m2)
-//
-// A few operations per element, so the floor is HBM traffic: x read and y
-// written once (x, dy read and dx written once in the backward). Every sum is
-// needed before the first output, so a sample is read twice; see the launchers
-// for how the second read comes out of L2.
-//
-// Numerics. A thread sums x - K and (x - K)^2 in float32 over its few dozen
-// rows, K being its first value of the channel: what a far-off K costs is
-// bounded by K's own share of the variance. Everything beyond a thread
-// (partial sums, mean, 1/std, the per-channel factors) is float64, so the sums
-// of different slices add without cancellation and the result does not depend
-// on the order the slices finish in: partial sums have slots of their own and
-// are added in a fixed order, with no float atomics.
-// z = x a + b with a = gamma r, b = beta - mu a split into two floats each,
-// which leaves the sign of z exact to ~2^-48: a rectifier's gradient jumps
-// there, and forward and backward must agree on the side.
-#include "feature_common.cuh"
+// Group norm: plan and launch, and the kernels for maps that the streamed ones
+// (norm_stream.cu) do not take: rows that are no whole number of aligned 16-byte
+// vectors, or wider than a CTA's threads.
+#include "norm_common.cuh"
 
 namespace lcb200 {
+
+bool stream_norm(const NormArgs& p, int dtype, bool backward, cudaStream_t s);
+int stream_norm_status(bool reset);
+int stream_stage_rows(int C, int dtype, bool backward);  // rows of a stage, at least 1
+
 namespace {
-
-constexpr int kT = 256;      // threads of a CTA
-constexpr int kUnroll = 4;   // rows a thread has in flight
-
-struct NormArgs {
-  const void* x;
-  const void* dy;
-  void* out;           // y or dx
-  const void* weight;  // [C] or null
-  const void* bias;    // [C] or null
-  int param_f32;       // weight/bias dtype: float32, else x's
-  double2* stats;      // [B, G] (mean, 1/std)
-  long long S;
-  int B, C, G, Cg;
-  int act;
-  float slope;
-  double eps;
-  int slices;           // slices of one sample
-  long long slice_rows;
-  // workspace
-  uint32_t* done;       // [B + 1] finished slices per sample, finished samples
-  double2* part;        // forward: [B, slices, G] (sum x, sum x^2)
-  float2* bpart;        // backward: [B, slices, C] (sum dz, sum dz (x - mu))
-  double2* sums;        // backward: [B, C] (A, X)
-  float4* coef;         // backward: [B, G] (mu, k2, k3, 0): dx = gamma r dz + k2 (x - mu) + k3
-  void* dweight;        // [C] or null
-  void* dbias;
-  DropArgs drop;
-};
-
-template <typename T>
-__device__ __forceinline__ double param(const void* p, int f32, int c, double none) {
-  if (!p) return none;
-  return f32 ? (double)__ldg(reinterpret_cast<const float*>(p) + c)
-             : (double)ldf(reinterpret_cast<const T*>(p) + c);
-}
-
-template <typename T>
-__device__ __forceinline__ void put_param(void* p, int f32, int c, double v) {
-  if (!p) return;
-  if (f32) reinterpret_cast<float*>(p)[c] = (float)v;
-  else stf(reinterpret_cast<T*>(p) + c, (float)v);
-}
-
-// sigma(z); exp(-z) overflowing to infinity gives 0.
-__device__ __forceinline__ float sigmoid(float z) { return __fdividef(1.f, 1.f + __expf(-z)); }
-
-__device__ __forceinline__ float act_value(float z, int act, float slope) {
-  if (act == LCB200_ACT_SILU) return z * sigmoid(z);
-  if (act == LCB200_ACT_RELU) return z < 0.f ? 0.f : z;  // NaN stays NaN
-  if (act == LCB200_ACT_LEAKY_RELU) return z < 0.f ? slope * z : z;
-  return z;
-}
-
-__device__ __forceinline__ float act_grad(float z, float g, int act, float slope) {
-  if (act == LCB200_ACT_SILU) {
-    const float sg = sigmoid(z);
-    return g * (sg * fmaf(z, 1.f - sg, 1.f));
-  }
-  if (act == LCB200_ACT_RELU) return z > 0.f ? g : 0.f;
-  if (act == LCB200_ACT_LEAKY_RELU) return z > 0.f ? g : slope * g;
-  return g;
-}
-
-// A thread's place in a CTA's rows x vector columns tiling.
-struct Place {
-  int nc;   // vector columns of the block starting at cb
-  int rp;   // rows a CTA covers per step
-  int col;  // vector column (of the whole row)
-  int row;
-  bool on;
-  __device__ __forceinline__ Place(int cols, int cb) {
-    nc = min(cols - cb, kT);
-    rp = kT / nc;
-    col = cb + threadIdx.x % nc;
-    row = threadIdx.x / nc;
-    on = row < rp;
-  }
-};
-
-__device__ __forceinline__ int pow2_below(int v) { return v < 1 ? 1 : 1 << (31 - __clz(v)); }
-
-__device__ __forceinline__ double2 lanes_sum(double2 v, int width) {
-  for (int o = width / 2; o > 0; o >>= 1) {
-    v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
-    v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
-  }
-  return v;
-}
-
-// (factor, offset) of the channel, z = x a + b, as unevaluated float pairs.
-struct Affine {
-  float ah, al, bh, bl;
-};
-template <typename T>
-__device__ __forceinline__ Affine affine(const NormArgs& p, double2 st, int c) {
-  const double a = param<T>(p.weight, p.param_f32, c, 1.0) * st.y;
-  const double b = param<T>(p.bias, p.param_f32, c, 0.0) - st.x * a;
-  Affine f;
-  f.ah = (float)a;
-  f.al = (float)(a - (double)f.ah);
-  f.bh = (float)b;
-  f.bl = (float)(b - (double)f.bh);
-  return f;
-}
-__device__ __forceinline__ float affine_z(const Affine& f, float x) {
-  return fmaf(x, f.ah, f.bh) + fmaf(x, f.al, f.bl);
-}
 
 // ---- forward, first pass: slice sums, and the sample's statistics -----------------
 template <typename T, int V>
@@ -238,55 +113,8 @@ __device__ void stats_slice(const NormArgs& p, int b, int j, double2* sm) {
   }
 }
 
-__device__ void stats_finish(const NormArgs& p, int b) {
-  const int width = min(32, max(1, pow2_below(min(p.slices, kT / min(p.G, kT)))));
-  const int lane = threadIdx.x % width;
-  const double inv = 1.0 / ((double)p.S * p.Cg);
-  for (int g0 = 0; g0 < p.G; g0 += kT / width) {
-    const int g = g0 + threadIdx.x / width;
-    double2 v = make_double2(0.0, 0.0);
-    if (g < p.G) {
-      const double2* src = p.part + (long long)b * p.slices * p.G + g;
-#pragma unroll 4
-      for (int j = lane; j < p.slices; j += width) {
-        const double2 e = __ldcg(src + (long long)j * p.G);
-        v.x += e.x;
-        v.y += e.y;
-      }
-    }
-    v = lanes_sum(v, width);
-    if (g < p.G && lane == 0) {
-      const double mean = v.x * inv;
-      double var = v.y * inv - mean * mean;
-      var = var < 0.0 ? 0.0 : var;  // rounding below zero; NaN stays
-      p.stats[(long long)b * p.G + g] = make_double2(mean, 1.0 / sqrt(var + p.eps));
-    }
-  }
-}
-
-// True in every thread of the CTA that finished last of `count` at *counter;
-// what the others wrote before is then visible.
-__device__ bool last_of(uint32_t* counter, uint32_t count) {
-  __shared__ int is_last;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    __threadfence();
-    is_last = atomicAdd(counter, 1u) == count - 1;
-    __threadfence();
-  }
-  __syncthreads();
-  return is_last;
-}
-
-template <typename T, int V>
-__global__ void __launch_bounds__(kT) norm_stats_kernel(NormArgs p) {
-  __shared__ double2 sm[kT * V];
-  const int b = blockIdx.x / p.slices, j = blockIdx.x % p.slices;
-  stats_slice<T, V>(p, b, j, sm);
-  if (last_of(p.done + b, p.slices)) stats_finish(p, b);
-}
-
 // ---- forward, second pass ------------------------------------------------------------
+// z = (x - muh) a + b with muh = mu rounded to float32 and b = beta - (mu - muh) a.
 template <typename T, int V, bool DROP>
 __device__ void apply_slice(const NormArgs& p, int b, int j) {
   const int cols = p.C / V;
@@ -297,11 +125,16 @@ __device__ void apply_slice(const NormArgs& p, int b, int j) {
   for (int cb = 0; cb < cols; cb += kT) {
     const Place at(cols, cb);
     if (!at.on) continue;
-    Affine f[V];
+    float mu[V], a[V], c[V];
     const int c0 = at.col * V;
 #pragma unroll
-    for (int v = 0; v < V; ++v)
-      f[v] = affine<T>(p, __ldcg(p.stats + (long long)b * p.G + (c0 + v) / p.Cg), c0 + v);
+    for (int v = 0; v < V; ++v) {
+      const double2 st = __ldcg(p.stats + (long long)b * p.G + (c0 + v) / p.Cg);
+      mu[v] = (float)st.x;
+      a[v] = (float)(param<T>(p.weight, p.param_f32, c0 + v, 1.0) * st.y);
+      c[v] = (float)(param<T>(p.bias, p.param_f32, c0 + v, 0.0) -
+                     (st.x - (double)mu[v]) * (double)a[v]);
+    }
     uint32_t keep = ~0u;
     if (DROP && p.drop.channel) keep = drop_keep<V>(ds, p.drop.threshold, (long long)b * p.C + c0);
     const T* src = reinterpret_cast<const T*>(p.x) + base + c0;
@@ -313,7 +146,7 @@ __device__ void apply_slice(const NormArgs& p, int b, int j) {
       if (DROP && !p.drop.channel) m = drop_keep<V>(ds, p.drop.threshold, base + r * p.C + c0);
 #pragma unroll
       for (int v = 0; v < V; ++v) {
-        x[v] = act_value(affine_z(f[v], x[v]), p.act, p.slope);
+        x[v] = act_value(fmaf(x[v] - mu[v], a[v], c[v]), p.act, p.slope);
         if (DROP) x[v] = (m >> v) & 1 ? x[v] * p.drop.factor : 0.f;
       }
       Vec<T, V>::store(dst + r * p.C, Vec<T, V>::pack(x));
@@ -329,12 +162,6 @@ __device__ void apply_slice(const NormArgs& p, int b, int j) {
     }
     for (; r < r1; r += step) one(Vec<T, V>::load_last(src + r * p.C), r);
   }
-}
-
-template <typename T, int V, bool DROP>
-__global__ void __launch_bounds__(kT) norm_apply_kernel(NormArgs p) {
-  drop_keep_stream(p.drop);
-  apply_slice<T, V, DROP>(p, blockIdx.x / p.slices, blockIdx.x % p.slices);
 }
 
 // ---- backward, first pass: per-channel sums of dz and dz (x - mu) --------------------
@@ -421,95 +248,6 @@ __device__ void grad_sums_slice(const NormArgs& p, int b, int j, float2* sm) {
   }
 }
 
-__device__ __forceinline__ double2 as_double2(float2 v) { return make_double2(v.x, v.y); }
-__device__ __forceinline__ double2 as_double2(double2 v) { return v; }
-
-// Column sums of an [n, C] matrix of pairs by the whole CTA, handed to
-// put(c, sum) by one thread per column; a fixed order for fixed sizes.
-template <typename P, typename F>
-__device__ void column_sums(const P* src, long long n, int C, double2* sm, F put) {
-  for (int cb = 0; cb < C; cb += kT) {
-    const int nc = min(C - cb, kT);
-    const int parts = (int)min((long long)(kT / nc), n);
-    const int c = threadIdx.x % nc, part = threadIdx.x / nc;
-    double2 v = make_double2(0.0, 0.0);
-    if (part < parts) {
-#pragma unroll 8
-      for (long long i = part; i < n; i += parts) {
-        const double2 e = as_double2(__ldcg(src + i * C + cb + c));
-        v.x += e.x;
-        v.y += e.y;
-      }
-    }
-    sm[threadIdx.x] = v;
-    __syncthreads();
-    if (part == 0) {
-      for (int k = 1; k < parts; ++k) {
-        v.x += sm[k * nc + c].x;
-        v.y += sm[k * nc + c].y;
-      }
-      put(cb + c, v);
-    }
-    __syncthreads();
-  }
-}
-
-template <typename T>
-__device__ void grad_finish(const NormArgs& p, int b, double2* sm) {
-  const double2* stats = p.stats + (long long)b * p.G;
-  double2* sums = p.sums + (long long)b * p.C;
-  column_sums(p.bpart + (long long)b * p.slices * p.C, p.slices, p.C, sm, [&](int c, double2 v) {
-    // the slices centred on mu rounded to float32
-    const double2 st = __ldg(stats + c / p.Cg);
-    sums[c] = make_double2(v.x, st.y * (v.y - (st.x - (double)(float)st.x) * v.x));
-  });
-  __threadfence_block();
-  __syncthreads();
-  const double inv = 1.0 / ((double)p.S * p.Cg);
-  const int width = min(32, max(1, pow2_below(min(p.Cg, kT / min(p.G, kT)))));
-  const int lane = threadIdx.x % width;
-  for (int g0 = 0; g0 < p.G; g0 += kT / width) {
-    const int g = g0 + threadIdx.x / width;
-    double2 v = make_double2(0.0, 0.0);
-    if (g < p.G) {
-      for (int i = lane; i < p.Cg; i += width) {
-        const int c = g * p.Cg + i;
-        const double w = param<T>(p.weight, p.param_f32, c, 1.0);
-        const double2 e = __ldcg(sums + c);
-        v.x += w * e.x;
-        v.y += w * e.y;
-      }
-    }
-    v = lanes_sum(v, width);
-    if (g < p.G && lane == 0) {
-      const double2 st = __ldg(stats + g);
-      // dx = gamma r dz - r m1 - r^2 m2 (x - mu), mu = muh + mul
-      const double k2 = -st.y * st.y * v.y * inv;
-      const double k3 = -st.y * v.x * inv - k2 * (st.x - (double)(float)st.x);
-      p.coef[(long long)b * p.G + g] = make_float4((float)st.x, (float)k2, (float)k3, 0.f);
-    }
-  }
-}
-
-template <typename T>
-__device__ void param_grads(const NormArgs& p, double2* sm) {
-  column_sums(p.sums, p.B, p.C, sm, [&](int c, double2 v) {
-    put_param<T>(p.dbias, p.param_f32, c, v.x);
-    put_param<T>(p.dweight, p.param_f32, c, v.y);
-  });
-}
-
-template <typename T, int V, bool DROP>
-__global__ void __launch_bounds__(kT) norm_grad_sums_kernel(NormArgs p) {
-  __shared__ __align__(16) float2 sm[kT * (V < 2 ? 2 : V)];  // also kT double2 sums
-  const int b = blockIdx.x / p.slices, j = blockIdx.x % p.slices;
-  grad_sums_slice<T, V, DROP>(p, b, j, sm);
-  double2* smd = reinterpret_cast<double2*>(sm);
-  if (!last_of(p.done + b, p.slices)) return;
-  grad_finish<T>(p, b, smd);
-  if (last_of(p.done + p.B, p.B)) param_grads<T>(p, smd);
-}
-
 // ---- backward, second pass --------------------------------------------------------------
 template <typename T, int V, bool DROP>
 __device__ void grad_input_slice(const NormArgs& p, int b, int j) {
@@ -568,75 +306,153 @@ __device__ void grad_input_slice(const NormArgs& p, int b, int j) {
   }
 }
 
+// ---- the kernels: both passes of every chunk --------------------------------------------
+template <typename F>
+__device__ void run_units(const NormArgs& p, F unit) {
+  __shared__ uint32_t s_next;
+  if (threadIdx.x == 0) s_next = atomicAdd(p.ticket, 1u);
+  __syncthreads();
+  uint32_t t = s_next;
+  while (t < p.tickets) {
+    uint32_t next = 0;
+    if (threadIdx.x == 0) next = atomicAdd(p.ticket, 1u);  // arrives during the unit
+    const Unit u = decode(p, t);
+    if (!unit(u.second, u.b, u.j)) return;
+    __syncthreads();
+    if (threadIdx.x == 0) s_next = next;
+    __syncthreads();
+    t = s_next;
+  }
+}
+
 template <typename T, int V, bool DROP>
-__global__ void __launch_bounds__(kT) norm_grad_input_kernel(NormArgs p) {
-  grad_input_slice<T, V, DROP>(p, blockIdx.x / p.slices, blockIdx.x % p.slices);
+__global__ void __launch_bounds__(kT, kOcc) norm_forward_kernel(NormArgs p) {
+  __shared__ double2 sm[kT * V];
+  drop_keep_stream(p.drop);
+  run_units(p, [&](bool second, int b, int j) {
+    if (!second) {
+      stats_slice<T, V>(p, b, j, sm);
+      if (finish_slice(p, b, j, p.part, p.G, sm, [&](int g, double2 t) {
+            p.stats[(long long)b * p.G + g] = finish_stats(p, t);
+          }))
+        publish(p.ready + b);
+      return true;
+    }
+    if (!wait_for(p.ready + b)) return false;
+    apply_slice<T, V, DROP>(p, b, j);
+    return true;
+  });
+}
+
+template <typename T, int V, bool DROP>
+__global__ void __launch_bounds__(kT, kOcc) norm_backward_kernel(NormArgs p) {
+  __shared__ __align__(16) float2 sm[kT * (V < 2 ? 2 : V)];  // also kT double2 sums
+  double2* smd = reinterpret_cast<double2*>(sm);
+  run_units(p, [&](bool second, int b, int j) {
+    if (!second) {
+      grad_sums_slice<T, V, DROP>(p, b, j, sm);
+      if (finish_slice(p, b, j, p.bpart, p.C, smd,
+                       [&](int c, double2 t) { finish_channel(p, b, c, t); })) {
+        finish_coef<T>(p, b);
+        publish(p.ready + b);
+        if (last_of(p.ticket + 1, p.B)) param_grads<T>(p, smd);
+      }
+      return true;
+    }
+    if (!wait_for(p.ready + b)) return false;
+    grad_input_slice<T, V, DROP>(p, b, j);
+    return true;
+  });
 }
 
 // ---- host ---------------------------------------------------------------------------------
-// Slices of a sample: about 64 KB of rows each, smaller while the batch does
-// not give every multiprocessor four of them, but at least four rows a thread
-// when rows are as narrow as the CTA.
-void plan_slices(int B, long long S, int C, int dtype, int* slices, long long* slice_rows) {
+// Widest rows of the streamed kernels: their per-group values, a double2 or float4
+// each, share a CTA's memory with the ring.
+constexpr int kStreamChannels = 2048;
+
+struct Plan {
+  int slices, fan, sets;
+  long long slice_rows;
+  uint32_t units, lag;
+  int ctas, stage_rows, chunk, chunks;
+  long long slots;
+  bool ok;
+};
+
+Plan make_plan(int B, long long S, int C, int dtype, bool backward) {
+  Plan q{};
   const size_t es = dtype_bytes(dtype);
-  const long long row_bytes = (long long)C * es;
-  const long long rp = std::max<long long>(1, kT * 16ll / row_bytes);  // rows of one CTA step
-  long long rows = std::max<long long>(1, 65536 / row_bytes);
-  const long long want = 4ll * device_sms();
-  const long long even = (long long)((double)S * B / want) + 1;
-  rows = std::min(rows, even);
-  rows = std::min(S, std::max(rows, 4 * rp));
-  *slice_rows = rows;
-  *slices = (int)((S + rows - 1) / rows);
+  const double maps = backward ? 2 : 1;
+  // plain kernels: units of 64 KB, fewer rows while the batch does not give every CTA
+  // two of them; a second pass 32 MB behind its first
+  const long long rp = std::max<long long>(1, (long long)kT * 16 / (long long)(C * es));
+  const long long step = 4 * rp, slots = (long long)device_sms() * kOcc;
+  const long long n = (long long)std::min<double>(4, (double)S * B / (double)(2 * slots * step));
+  q.slice_rows = std::min<long long>(S, std::max<long long>(1, n) * step);
+  const long long slices = (S + q.slice_rows - 1) / q.slice_rows, units = slices * B;
+  q.slices = (int)slices;
+  q.units = (uint32_t)units;
+  q.lag = (uint32_t)std::min<long long>(
+      units, slices + (long long)((32 << 20) / (maps * q.slice_rows * C * es)));
+  // streamed kernels: chunks of up to 160 MB. L2 holds less of that, but the exchange of
+  // a chunk's sums costs 5 to 6 us: 8 x 135 x 240 x 256 float16, forward and backward,
+  // takes 242 us in chunks of 40 MB, 223 of 72 and 201 of 200 MB
+  const double target = 160 << 20;
+  const double total = maps * (double)S * B * C * es;
+  const long long k = std::min<long long>(B, (long long)(total / target) + 1);
+  q.chunk = (int)((B + k - 1) / k);
+  q.chunks = (B + q.chunk - 1) / q.chunk;
+  q.stage_rows = stream_stage_rows(C, dtype, backward);
+  q.ctas = device_sms();
+  q.ctas = std::min(q.ctas, chunk_parts(q.chunk * S, q.stage_rows, q.ctas));
+  q.slots = (long long)q.chunks * (2ll * q.ctas + q.chunk);
+  q.ok = slices < (1ll << 30) && units < 2000000000ll && S * q.chunk < (1ll << 40) &&
+         q.slots < (1ll << 31);
+  q.fan = 1;
+  while ((long long)q.fan * q.fan < slices) ++q.fan;
+  q.sets = (int)((slices + q.fan - 1) / q.fan);
+  return q;
 }
 
-struct Layout {
-  size_t done, part, sums, coef, total;
+struct Layout {  // byte offsets
+  size_t flags, part, plain, set_part, bpart, sums, coef, total;
 };
-Layout layout(int B, int C, int G, int slices, bool backward) {
-  auto up = [](size_t v) { return (v + 255) / 256 * 256; };
-  Layout l{};
+// [0, flags): counters of the plain kernels, from 0. [part, plain): entries of the
+// streamed kernels, from all ones.
+Layout layout(const Plan& q, int B, int C, int G, bool backward) {
   size_t at = 0;
-  l.done = at;
-  at = up(at + sizeof(uint32_t) * ((size_t)B + 1));
-  l.part = at;
-  at = up(at + (backward ? sizeof(float2) * (size_t)C : sizeof(double2) * (size_t)G) * B * slices);
+  auto take = [&](size_t bytes) {
+    const size_t from = at;
+    at = (at + bytes + 255) / 256 * 256;
+    return from;
+  };
+  Layout l{};
+  take(l.flags = sizeof(uint32_t) * (2 + (2 + (size_t)q.sets) * B));
+  l.part = take(sizeof(double2) * (size_t)G * std::max<size_t>(q.units, q.slots));
+  l.plain = at;
+  l.set_part = take(sizeof(double2) * (size_t)(backward ? C : G) * B * q.sets);
   if (backward) {
-    l.sums = at;
-    at = up(at + sizeof(double2) * (size_t)B * C);
-    l.coef = at;
-    at = up(at + sizeof(float4) * (size_t)B * G);
+    l.bpart = take(sizeof(float2) * (size_t)C * q.units);
+    l.sums = take(sizeof(double2) * (size_t)C * std::max(B, q.ctas));
+    l.coef = take(sizeof(float4) * (size_t)B * G);
   }
   l.total = at;
   return l;
 }
 
 template <typename T, int V, bool DROP>
-bool launch_forward(const NormArgs& p, cudaStream_t s) {
-  const unsigned grid = (unsigned)((long long)p.B * p.slices);
-  norm_stats_kernel<T, V><<<grid, kT, 0, s>>>(p);
-  norm_apply_kernel<T, V, DROP><<<grid, kT, 0, s>>>(p);
-  count_launch(2);
-  return check_launch("group norm");
-}
-
-template <typename T, int V, bool DROP>
-bool launch_backward(const NormArgs& p, cudaStream_t s) {
-  const unsigned grid = (unsigned)((long long)p.B * p.slices);
-  norm_grad_sums_kernel<T, V, DROP><<<grid, kT, 0, s>>>(p);
+bool launch_kernel(const NormArgs& p, bool backward, cudaStream_t s) {
+  const unsigned grid = std::min<unsigned>(p.tickets, (unsigned)(device_sms() * kOcc));
+  if (backward) norm_backward_kernel<T, V, DROP><<<grid, kT, 0, s>>>(p);
+  else norm_forward_kernel<T, V, DROP><<<grid, kT, 0, s>>>(p);
   count_launch();
-  if (p.out) {
-    norm_grad_input_kernel<T, V, DROP><<<grid, kT, 0, s>>>(p);
-    count_launch();
-  }
-  return check_launch("group norm backward");
+  return check_launch(backward ? "group norm backward" : "group norm");
 }
 
 template <typename T, int V>
 bool launch_v(const NormArgs& p, bool backward, cudaStream_t s) {
-  const bool drop = p.drop.threshold != 0;
-  if (backward) return drop ? launch_backward<T, V, true>(p, s) : launch_backward<T, V, false>(p, s);
-  return drop ? launch_forward<T, V, true>(p, s) : launch_forward<T, V, false>(p, s);
+  return p.drop.threshold != 0 ? launch_kernel<T, V, true>(p, backward, s)
+                               : launch_kernel<T, V, false>(p, backward, s);
 }
 
 template <typename T>
@@ -658,10 +474,8 @@ bool launch(const NormArgs& p, int dtype, bool backward, cudaStream_t s) {
 }  // namespace
 
 size_t feature_norm_workspace(int B, long long S, int C, int G, int dtype, bool backward) {
-  int slices;
-  long long rows;
-  plan_slices(B, S, C, dtype, &slices, &rows);
-  return layout(B, C, G, slices, backward).total;
+  const Plan q = make_plan(B, S, C, dtype, backward);
+  return q.ok ? layout(q, B, C, G, backward).total : 0;
 }
 
 bool feature_norm(const void* x, const void* dy, const void* weight, const void* bias, void* out,
@@ -669,6 +483,18 @@ bool feature_norm(const void* x, const void* dy, const void* weight, const void*
                   int dtype, bool param_f32, double eps, int act, float slope,
                   const DropArgs& drop, void* ws, size_t ws_bytes, bool backward,
                   cudaStream_t s) {
+  const Plan q = make_plan(B, S, C, dtype, backward);
+  if (!q.ok) {
+    set_error("group norm: too many samples");
+    return false;
+  }
+  const Layout l = layout(q, B, C, G, backward);
+  if (!ws || ws_bytes < l.total || (reinterpret_cast<uintptr_t>(ws) & 15)) {
+    set_error("group norm: needs a 16-byte aligned workspace of " + std::to_string(l.total) +
+              " B, got " + std::to_string(ws_bytes));
+    return false;
+  }
+  uint8_t* w = static_cast<uint8_t*>(ws);
   NormArgs p{};
   p.x = x;
   p.dy = dy;
@@ -685,29 +511,39 @@ bool feature_norm(const void* x, const void* dy, const void* weight, const void*
   p.act = act;
   p.slope = slope;
   p.eps = eps;
+  p.slices = q.slices;
+  p.slice_rows = q.slice_rows;
+  p.fan = q.fan;
+  p.sets = q.sets;
+  p.units = q.units;
+  p.lag = q.lag;
+  p.ctas = q.ctas;
+  p.stage_rows = q.stage_rows;
+  p.chunk = q.chunk;
+  p.chunks = q.chunks;
+  p.tickets = out ? 2 * q.units : q.units;
+  const int full = 16 / (int)dtype_bytes(dtype);
+  const bool stream = C <= kStreamChannels && vec_width(dtype, C, x, out, dy) == full;
+  p.ticket = reinterpret_cast<uint32_t*>(w);
+  p.done = p.ticket + 2;
+  p.sets_done = p.done + (size_t)B * q.sets;
+  p.ready = p.sets_done + B;
+  p.part = reinterpret_cast<double2*>(w + l.part);
+  p.bpart = reinterpret_cast<float2*>(w + l.bpart);
+  p.set_part = reinterpret_cast<double2*>(w + l.set_part);
+  p.sums = reinterpret_cast<double2*>(w + l.sums);
+  p.coef = reinterpret_cast<float4*>(w + l.coef);
   p.dweight = dweight;
   p.dbias = dbias;
   p.drop = drop;
-  plan_slices(B, S, C, dtype, &p.slices, &p.slice_rows);
-  if ((long long)B * p.slices > 0x7fffffffll) {
-    set_error("group norm: too many samples");
-    return false;
-  }
-  const Layout l = layout(B, C, G, p.slices, backward);
-  if (!ws || ws_bytes < l.total || (reinterpret_cast<uintptr_t>(ws) & 15)) {
-    set_error("group norm: needs a 16-byte aligned workspace of " + std::to_string(l.total) +
-              " B, got " + std::to_string(ws_bytes));
-    return false;
-  }
-  uint8_t* w = static_cast<uint8_t*>(ws);
-  p.done = reinterpret_cast<uint32_t*>(w + l.done);
-  p.part = reinterpret_cast<double2*>(w + l.part);
-  p.bpart = reinterpret_cast<float2*>(w + l.part);
-  p.sums = reinterpret_cast<double2*>(w + l.sums);
-  p.coef = reinterpret_cast<float4*>(w + l.coef);
-  if (cudaMemsetAsync(p.done, 0, sizeof(uint32_t) * ((size_t)B + 1), s) != cudaSuccess)
+  if ((stream ? cudaMemsetAsync(w + l.part, 0xff, sizeof(double2) * (size_t)G * q.slots, s)
+              : cudaMemsetAsync(w, 0, l.flags, s)) != cudaSuccess)
     return check_launch("group norm: memset of the counters");
-  return launch(p, dtype, backward, s);
+  return stream ? stream_norm(p, dtype, backward, s) : launch(p, dtype, backward, s);
+}
+
+int feature_device_status(bool reset) {
+  return read_norm_status(reset) | stream_norm_status(reset);
 }
 
 }  // namespace lcb200

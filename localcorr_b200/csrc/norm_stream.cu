@@ -1,0 +1,904 @@
+// Group norm for rows of aligned 16-byte vectors, no wider than a CTA's threads.
+//
+// HBM bound, so the aim is loads that never pause and few instructions a vector
+// (a pass of 16-bit maps has about 90 issue slots per 16 bytes read and written
+// before it falls behind HBM). One CTA per multiprocessor. The rows of a chunk of
+// samples are divided evenly over the CTAs; a CTA makes its first pass (sums) over its
+// rows of a chunk and later its second pass (outputs), by then out of L2. A producer
+// warp copies the rows into a ring of stages with bulk copies, running on across
+// passes; the other warps do the arithmetic, two float32 operations an instruction.
+//
+// Order of a CTA: first(0) | first(1) a, second(0), first(1) b | first(2) a, second(1),
+// first(2) b | ... | second(last): while a chunk's sums travel between the CTAs,
+// everybody is in half a first pass of the next chunk.
+//
+// The sums travel through 16-byte entries that are written whole and start out as all
+// ones: a reader polls the entry itself, so no fence, counter or flag stands between a
+// sum and its reader, and every CTA adds up the entries of its samples itself, one
+// round trip after the last of them is written. Waiting needs every CTA resident: the
+// kernels are launched cooperatively. (Dynamic units finished by the last arriver of
+// an atomic counter made the statistics wait 13 to 18 us: a round trip takes 2 to 3 us
+// while the copies saturate HBM.)
+#include "norm_common.cuh"
+#include "tc_ptx.cuh"
+
+namespace lcb200 {
+namespace {
+
+constexpr int kS = 512;          // arithmetic threads
+constexpr int kBlock = kS + 32;  // and the producer warp
+// Vectors of a thread per stage and map: 32 KB stages. A stage costs about 570 cycles
+// from barrier to barrier however small it is: reading 531 MB with one CTA a
+// multiprocessor takes 264 us in 4 KB stages, 141 in 8, 90 in 16 and 86 in 32 KB.
+template <int NM> constexpr int kVecs = 4 / NM;
+
+__device__ __forceinline__ void stream_sync() {
+  asm volatile("bar.sync 1, %0;" ::"n"(kS) : "memory");
+}
+
+__device__ __forceinline__ uint64_t bits(float2 v) { return *reinterpret_cast<uint64_t*>(&v); }
+__device__ __forceinline__ float2 pair(uint64_t v) { return *reinterpret_cast<float2*>(&v); }
+__device__ __forceinline__ float2 twice(float v) { return make_float2(v, v); }
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(bits(a)), "l"(bits(b)));
+  return pair(r);
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(bits(a)), "l"(bits(b)));
+  return pair(r);
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(bits(a)), "l"(bits(b)), "l"(bits(c)));
+  return pair(r);
+}
+
+// One 16-byte vector as float pairs, and back.
+template <typename T> struct Vec2;
+template <> struct Vec2<float> {
+  static __device__ __forceinline__ void unpack(uint4 r, float2 (&f)[2]) {
+    f[0] = make_float2(__uint_as_float(r.x), __uint_as_float(r.y));
+    f[1] = make_float2(__uint_as_float(r.z), __uint_as_float(r.w));
+  }
+  static __device__ __forceinline__ uint4 pack(const float2 (&f)[2]) {
+    return make_uint4(__float_as_uint(f[0].x), __float_as_uint(f[0].y), __float_as_uint(f[1].x),
+                      __float_as_uint(f[1].y));
+  }
+  static __device__ __forceinline__ uint32_t relu(uint32_t v) {  // NaN stays
+    float r;
+    asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(r) : "f"(__uint_as_float(v)));
+    return __float_as_uint(r);
+  }
+};
+template <> struct Vec2<__half> {
+  static __device__ __forceinline__ void unpack(uint4 r, float2 (&f)[4]) {
+    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+  }
+  static __device__ __forceinline__ uint4 pack(const float2 (&f)[4]) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) *reinterpret_cast<__half2*>(&w[i]) = __float22half2_rn(f[i]);
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  static __device__ __forceinline__ uint32_t relu(uint32_t v) {
+    uint32_t r;
+    asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(v), "r"(0u));
+    return r;
+  }
+};
+template <> struct Vec2<__nv_bfloat16> {
+  static __device__ __forceinline__ void unpack(uint4 r, float2 (&f)[4]) {
+    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      f[i] = make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+  }
+  static __device__ __forceinline__ uint4 pack(const float2 (&f)[4]) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      *reinterpret_cast<__nv_bfloat162*>(&w[i]) = __float22bfloat162_rn(f[i]);
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  static __device__ __forceinline__ uint32_t relu(uint32_t v) {
+    uint32_t r;
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(v), "r"(0u));
+    return r;
+  }
+};
+
+__device__ __forceinline__ void keep2(float2& v, uint32_t m) {
+  v.x = m & 1 ? v.x : 0.f;
+  v.y = m & 2 ? v.y : 0.f;
+}
+
+// ---- entries --------------------------------------------------------------------------
+// 16 bytes as two words; all ones: not written yet.
+struct Entry {
+  unsigned long long lo, hi;
+  __device__ __forceinline__ bool ready() const { return (lo & hi) != ~0ull; }
+};
+__device__ __forceinline__ Entry entry_of(double2 v) {
+  Entry e{(unsigned long long)__double_as_longlong(v.x),
+          (unsigned long long)__double_as_longlong(v.y)};
+  if (!e.ready()) e.lo = 0x7ff8000000000000ull;  // a NaN like any other
+  return e;
+}
+__device__ __forceinline__ double2 pair_of(const Entry& e) {
+  return make_double2(__longlong_as_double((long long)e.lo), __longlong_as_double((long long)e.hi));
+}
+__device__ __forceinline__ Entry get(const void* p) {
+  Entry e;
+  asm volatile(
+      "{\n\t.reg .b128 v;\n\tld.relaxed.gpu.global.b128 v, [%2];\n\tmov.b128 {%0, %1}, v;\n\t}"
+      : "=l"(e.lo), "=l"(e.hi)
+      : "l"(p)
+      : "memory");
+  return e;
+}
+__device__ __forceinline__ void put(void* p, const Entry& e) {
+  asm volatile(
+      "{\n\t.reg .b128 v;\n\tmov.b128 v, {%1, %2};\n\tst.relaxed.gpu.global.b128 [%0], v;\n\t}" ::"l"(p),
+      "l"(e.lo), "l"(e.hi)
+      : "memory");
+}
+
+// ---- the ring ------------------------------------------------------------------------
+struct StageInfo {
+  long long off;  // element offset of the stage's first row
+  int rows;       // of the stage
+  int b;          // sample
+  int seg;        // slot of the segment's sums
+  int seg_rows;
+  int flags;
+};
+enum : int { kSecond = 1, kLast = 2, kEnd = 4, kTop = 8 };  // kTop: starts the sample
+
+template <int NM, int STAGES>
+struct RingShared {
+  uint4 data[STAGES][NM][kVecs<NM> * kS];
+  uint64_t full[STAGES], empty[STAGES];
+  StageInfo info[STAGES];
+  int abort;
+};
+
+__device__ __forceinline__ void bulk_copy(void* dst, const void* src, uint32_t bytes,
+                                          uint64_t* bar, uint64_t policy) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint"
+      " [%0], [%1], %2, [%3], %4;" ::"r"(tc::smem_u32(dst)),
+      "l"(src), "r"(bytes), "r"(tc::smem_u32(bar)), "l"(policy)
+      : "memory");
+}
+
+template <int NM, int STAGES>
+__device__ void ring_init(RingShared<NM, STAGES>& r) {
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < STAGES; ++i) {
+      tc::mbar_init(&r.full[i], 1);
+      tc::mbar_init(&r.empty[i], kS / 32);
+    }
+    r.abort = 0;
+    tc::fence_mbar_init();
+  }
+  __syncthreads();
+}
+
+// ---- the division of the work -----------------------------------------------------------
+// Chunk k: samples [k m, k m + count), its rows cut into `parts` runs of equal length
+// (to a row), run q starting at row q rows / parts. CTA i has run i, or 2 i and 2 i + 1
+// (its halves a and b). A run is cut again where a sample ends: segments, the s-th
+// sample's in run q with slot q + s of the chunk's.
+struct Chunk {
+  int first, count, parts;
+  long long rows;
+  long long slots;  // of the chunks before
+  __device__ __forceinline__ Chunk(const NormArgs& p, int k) {
+    first = k * p.chunk;
+    count = min(p.chunk, p.B - first);
+    rows = count * p.S;
+    parts = chunk_parts(rows, p.stage_rows, p.ctas);
+    slots = (long long)k * (2 * p.ctas + p.chunk);
+  }
+  __device__ __forceinline__ long long start(int q) const {
+    return (long long)((unsigned long long)q * (unsigned long long)rows / (unsigned)parts);
+  }
+  // the run that holds row r
+  __device__ __forceinline__ int run_of(long long r) const {
+    return (int)(((unsigned long long)(r + 1) * (unsigned)parts - 1) / (unsigned long long)rows);
+  }
+  __device__ __forceinline__ bool halves(const NormArgs& p) const { return parts > p.ctas; }
+};
+
+// seg(sample of the chunk, first row, end row within the sample) for rows
+// [start, end) of a chunk.
+template <typename F>
+__device__ __forceinline__ void each_segment(const NormArgs& p, long long start, long long end,
+                                             F seg) {
+  int s = (int)(start / p.S);
+  long long r = start - s * p.S;
+  for (long long left = end - start; left > 0; ++s, r = 0) {
+    const long long stop = min(p.S, r + left);
+    seg(s, r, stop);
+    left -= stop - r;
+  }
+}
+
+// One thread. A segment is a run of whole rows, so its bytes are contiguous.
+template <typename T, int NM, int STAGES>
+__device__ void produce(const NormArgs& p, RingShared<NM, STAGES>& r, const T* m0, const T* m1) {
+  uint64_t stay, go;  // a first pass's rows are read again, a second pass's are not
+  asm volatile("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(stay));
+  asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(go));
+  uint32_t n = 0;  // stages issued
+  bool good = true;
+  auto claim = [&]() {
+    return tc::mbar_wait(&r.empty[n % STAGES], ((n / STAGES) & 1) ^ 1, &r.abort);
+  };
+  // runs q to q + runs - 1, as one
+  auto run = [&](const Chunk& c, int q, int runs, bool second) {
+    if (q >= c.parts) return;
+    const uint64_t policy = second ? go : stay;
+    each_segment(p, c.start(q), c.start(q + runs), [&](int s, long long row, long long end) {
+      const int seg = (int)(c.slots + q + s), seg_rows = (int)(end - row);
+      const int flags = (second ? kSecond : 0) | (row == 0 ? kTop : 0);
+      long long off = ((long long)(c.first + s) * p.S + row) * p.C;
+      while (row < end && good && (good = claim())) {
+        const int at = n % STAGES;
+        const int rows = (int)min((long long)p.stage_rows, end - row);
+        const uint32_t bytes = (uint32_t)(rows * p.C * sizeof(T));
+        row += rows;
+        r.info[at] = StageInfo{off, rows, c.first + s, seg, seg_rows,
+                               flags | (row == end ? kLast : 0)};
+        tc::mbar_arrive_expect_tx(&r.full[at], bytes * NM);
+        bulk_copy(r.data[at][0], m0 + off, bytes, &r.full[at], policy);
+        if (NM > 1) bulk_copy(r.data[at][NM - 1], m1 + off, bytes, &r.full[at], policy);
+        off += (long long)rows * p.C;
+        ++n;
+      }
+    });
+  };
+  const int i = blockIdx.x;
+  for (int k = 0; k <= p.chunks && good; ++k) {
+    const bool some = k < p.chunks;
+    const Chunk c(p, some ? k : 0);
+    const bool two = c.halves(p);
+    if (some) run(c, two ? 2 * i : i, 1, false);
+    if (k > 0 && p.out) {
+      const Chunk before(p, k - 1);
+      if (before.halves(p)) run(before, 2 * i, 2, true);
+      else run(before, i, 1, true);
+    }
+    if (some && two) run(c, 2 * i + 1, 1, false);
+  }
+  if (good && claim()) {
+    r.info[n % STAGES].flags = kEnd;
+    tc::mbar_arrive(&r.full[n % STAGES]);
+  } else {  // gave up: no copy may be in flight when the CTA ends
+    for (uint32_t k = n > STAGES ? n - STAGES : 0; k < n; ++k)
+      tc::mbar_wait_drain(&r.full[k % STAGES], (k / STAGES) & 1);
+  }
+}
+
+// The arithmetic warps' side.
+template <int NM, int STAGES>
+struct Consumer {
+  RingShared<NM, STAGES>& r;
+  uint32_t n = 0;
+  StageInfo now{};
+
+  __device__ __forceinline__ explicit Consumer(RingShared<NM, STAGES>& ring) : r(ring) {}
+  // Waits for the next stage; false at the end or when a wait ran out.
+  __device__ __forceinline__ bool open() {
+    if (!tc::mbar_wait(&r.full[n % STAGES], (n / STAGES) & 1, &r.abort)) {
+      atomicExch(&norm_status, 1);
+      return false;
+    }
+    now = r.info[n % STAGES];
+    return !(now.flags & kEnd);
+  }
+  __device__ __forceinline__ const uint4* map(int m) const { return r.data[n % STAGES][m]; }
+  __device__ __forceinline__ void close() {
+    __syncwarp();
+    if (threadIdx.x % 32 == 0) tc::mbar_arrive(&r.empty[n % STAGES]);
+    ++n;
+  }
+};
+
+// Calls row(i-th vector of the stage's map 0, row) for this thread's rows of a stage.
+template <int VECS, typename F>
+__device__ __forceinline__ void stage_rows(const Place& at, int rows, F row) {
+  const int active = at.nc * at.rp;
+  if (rows == at.rp * VECS) {
+    if (at.on) {
+#pragma unroll
+      for (int i = 0; i < VECS; ++i) row(threadIdx.x + i * active, at.row + i * at.rp);
+    }
+  } else if (at.on) {
+#pragma unroll 1
+    for (int i = 0; at.row + i * at.rp < rows; ++i)
+      row(threadIdx.x + i * active, at.row + i * at.rp);
+  }
+}
+
+// ---- the sums of a sample ------------------------------------------------------------
+// Polls an entry that was not ready; gives up after two seconds, or when another
+// thread of the CTA did.
+__device__ __forceinline__ Entry poll(const void* p, volatile int* abort) {
+  const uint64_t t0 = tc::globaltimer();
+  for (uint32_t i = 1;; ++i) {
+    const Entry e = get(p);
+    if (e.ready()) return e;
+    if (i % 32 == 0 && (*abort || tc::globaltimer() - t0 > 2000000000ull)) {
+      *abort = 1;
+      atomicExch(&norm_status, 1);
+      return Entry{0, 0};
+    }
+    __nanosleep(40);
+  }
+}
+// done(g, sum of the sample's entries of group g) by one thread per group, in an order
+// that only the sizes decide. All arithmetic threads take part, `width` of them a
+// group, with up to kFlight entries each in flight.
+template <typename F>
+__device__ __forceinline__ void sample_sums(const NormArgs& p, int b, volatile int* abort,
+                                            F done) {
+  constexpr int kFlight = 8;
+  const Chunk c(p, b / p.chunk);
+  const int s = b - c.first;
+  const int first = c.run_of(s * p.S), runs = c.run_of((s + 1) * p.S - 1) - first + 1;
+  const int width = p.G >= kS ? 1 : min(32, pow2_below(kS / p.G));
+  const int lane = threadIdx.x % width;
+  for (int g0 = 0; g0 < p.G; g0 += kS / width) {
+    const int g = g0 + threadIdx.x / width;
+    double2 v = make_double2(0.0, 0.0);
+    if (g < p.G) {
+      const double2* src = p.part + (c.slots + first + s) * p.G + g;
+#pragma unroll 1
+      for (int at = lane; at < runs; at += kFlight * width) {
+        Entry e[kFlight];
+#pragma unroll
+        for (int u = 0; u < kFlight; ++u)  // past the end: the last one again
+          e[u] = get(src + (long long)min(at + u * width, runs - 1) * p.G);
+#pragma unroll
+        for (int u = 0; u < kFlight; ++u) {
+          if (at + u * width < runs) {
+            if (!e[u].ready()) e[u] = poll(src + (long long)(at + u * width) * p.G, abort);
+            const double2 d = pair_of(e[u]);
+            v.x += d.x;
+            v.y += d.y;
+          }
+        }
+      }
+    }
+    v = lanes_sum(v, width);
+    if (g < p.G && lane == 0) done(g, v);
+  }
+}
+
+// ---- forward -------------------------------------------------------------------------
+// WHOLE: a vector lies in one group, so its V channels share the sums' K.
+template <typename T, bool WHOLE>
+struct ForwardShared {
+  static constexpr int kV = 16 / sizeof(T), kStages = 4;
+  RingShared<1, kStages> ring;
+  float sums[3][kS * (WHOLE ? 1 : kV)];  // K, sum (x - K), sum (x - K)^2 of each thread
+  double2 stats[1];                      // [G] of the second pass's sample
+};
+
+template <typename T, bool WHOLE, typename C>
+__device__ __forceinline__ bool stats_unit(const NormArgs& p, const Place& at, C& in,
+                                           ForwardShared<T, WHOLE>& sh) {
+  constexpr int V = 16 / sizeof(T), N = WHOLE ? 1 : V;
+  float2 k[V / 2], s[V / 2], q[V / 2];  // k: minus K
+#pragma unroll
+  for (int v = 0; v < V / 2; ++v) s[v] = q[v] = k[v] = twice(0.f);
+  const int seg = in.now.seg, rows = in.now.seg_rows;
+  bool first = true;
+  for (;;) {
+    const uint4* data = in.map(0);
+    if (first && at.on && at.row < in.now.rows) {
+      float2 f[V / 2];
+      Vec2<T>::unpack(data[threadIdx.x], f);
+#pragma unroll
+      for (int v = 0; v < V / 2; ++v)
+        k[v] = WHOLE ? twice(-f[0].x) : make_float2(-f[v].x, -f[v].y);
+    }
+    first = false;
+    stage_rows<kVecs<1>>(at, in.now.rows, [&](int i, int) {
+      float2 f[V / 2];
+      Vec2<T>::unpack(data[i], f);
+#pragma unroll
+      for (int v = 0; v < V / 2; ++v) {
+        const float2 d = add2(f[v], k[v]);
+        s[v] = add2(s[v], d);
+        q[v] = fma2(d, d, q[v]);
+      }
+    });
+    const bool last = in.now.flags & kLast;
+    in.close();
+    if (last) break;
+    if (!in.open()) return false;
+  }
+  if (WHOLE) {
+    float2 ss = s[0], qq = q[0];
+#pragma unroll
+    for (int v = 1; v < V / 2; ++v) {
+      ss = add2(ss, s[v]);
+      qq = add2(qq, q[v]);
+    }
+    sh.sums[0][threadIdx.x] = -k[0].x;
+    sh.sums[1][threadIdx.x] = ss.x + ss.y;
+    sh.sums[2][threadIdx.x] = qq.x + qq.y;
+  } else {
+#pragma unroll
+    for (int v = 0; v < V / 2; ++v) {
+      const int at2 = threadIdx.x * V / 2 + v;
+      reinterpret_cast<float2*>(sh.sums[0])[at2] = make_float2(-k[v].x, -k[v].y);
+      reinterpret_cast<float2*>(sh.sums[1])[at2] = s[v];
+      reinterpret_cast<float2*>(sh.sums[2])[at2] = q[v];
+    }
+  }
+  stream_sync();
+  // One group by `width` lanes: sum x = s + n K, sum x^2 = q + 2 K s + n K^2 in
+  // float64, n values an entry.
+  const int ne = at.nc * N, gw = p.Cg * N / V, full = rows / at.rp, rest = rows % at.rp;
+  const int width = min(32, max(1, pow2_below(min(at.rp * gw, kS / min(p.G, kS)))));
+  const int lane = threadIdx.x % width;
+  for (int g0 = 0; g0 < p.G; g0 += kS / width) {
+    const int g = g0 + threadIdx.x / width;
+    double2 t = make_double2(0.0, 0.0);
+    if (g < p.G) {
+      for (int i = lane; i < at.rp * gw; i += width) {
+        const int r = i / gw, e = r * ne + g * gw + (i - r * gw);
+        const int steps = full + (r < rest);
+        if (steps > 0) {
+          const double n = steps * (V / N);
+          const double k = sh.sums[0][e], s = sh.sums[1][e], q = sh.sums[2][e];
+          t.x += s + n * k;
+          t.y += q + k * (2.0 * s + n * k);
+        }
+      }
+    }
+    t = lanes_sum(t, width);
+    if (g < p.G && lane == 0) put(p.part + (long long)seg * p.G + g, entry_of(t));
+  }
+  stream_sync();  // the sums have been read
+  return true;
+}
+
+template <typename T, bool WHOLE, bool DROP, typename C>
+__device__ __forceinline__ bool apply_unit(const NormArgs& p, const Place& at, C& in,
+                                           double2* stats) {
+  constexpr int V = 16 / sizeof(T), N = WHOLE ? 1 : V / 2;
+  const int b = in.now.b, c0 = at.col * V;
+  const bool top = in.now.flags & kTop;
+  stream_sync();  // the last sample's have been read
+  sample_sums(p, b, &in.r.abort, [&](int g, double2 t) {
+    stats[g] = finish_stats(p, t);
+    if (top) p.stats[(long long)b * p.G + g] = stats[g];
+  });
+  stream_sync();
+  // z = (x - mu) a + c, mu rounded to float32, c = beta - (what the rounding left) a
+  float2 mu[N], a[V / 2], c[V / 2];  // mu: minus mu
+  float rstd = 0.f, left = 0.f;
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    if (!WHOLE || v == 0) {
+      const double2 st = stats[(c0 + v) / p.Cg];
+      const float m = -(float)st.x;
+      left = (float)(st.x + (double)m);
+      rstd = (float)st.y;
+      if (WHOLE) mu[0] = twice(m);
+      else (v & 1 ? mu[v / 2 % N].y : mu[v / 2 % N].x) = m;
+    }
+    const float av = param_f<T>(p.weight, p.param_f32, c0 + v, 1.f) * rstd;
+    const float cv = fmaf(-left, av, param_f<T>(p.bias, p.param_f32, c0 + v, 0.f));
+    (v & 1 ? a[v / 2].y : a[v / 2].x) = av;
+    (v & 1 ? c[v / 2].y : c[v / 2].x) = cv;
+  }
+  DropStream ds;
+  uint32_t keep = ~0u;
+  if (DROP) {
+    ds = drop_stream(p.drop);
+    if (p.drop.channel) keep = drop_keep<V>(ds, p.drop.threshold, (long long)b * p.C + c0);
+  }
+  T* dst = reinterpret_cast<T*>(p.out);
+  const int act = p.act;
+  for (;;) {
+    const uint4* data = in.map(0);
+    const long long first = in.now.off + c0;
+    stage_rows<kVecs<1>>(at, in.now.rows, [&](int i, int row) {
+      float2 x[V / 2];
+      Vec2<T>::unpack(data[i], x);
+      const long long e = first + (long long)row * p.C;
+      if (DROP && !p.drop.channel) keep = drop_keep<V>(ds, p.drop.threshold, e);
+#pragma unroll
+      for (int v = 0; v < V / 2; ++v) x[v] = fma2(add2(x[v], mu[WHOLE ? 0 : v % N]), a[v], c[v]);
+      if (act == LCB200_ACT_SILU) {
+#pragma unroll
+        for (int v = 0; v < V / 2; ++v) {
+          x[v].x *= sigmoid(x[v].x);
+          x[v].y *= sigmoid(x[v].y);
+        }
+      } else if (act == LCB200_ACT_LEAKY_RELU) {
+#pragma unroll
+        for (int v = 0; v < V / 2; ++v) {
+          x[v].x *= x[v].x < 0.f ? p.slope : 1.f;
+          x[v].y *= x[v].y < 0.f ? p.slope : 1.f;
+        }
+      }
+      if (DROP) {
+#pragma unroll
+        for (int v = 0; v < V / 2; ++v) {
+          x[v] = mul2(x[v], twice(p.drop.factor));
+          keep2(x[v], keep >> (2 * v));
+        }
+      }
+      uint4 r = Vec2<T>::pack(x);
+      if (act == LCB200_ACT_RELU) {  // commutes with the factor and the rounding
+        r.x = Vec2<T>::relu(r.x);
+        r.y = Vec2<T>::relu(r.y);
+        r.z = Vec2<T>::relu(r.z);
+        r.w = Vec2<T>::relu(r.w);
+      }
+      __stcs(reinterpret_cast<uint4*>(dst + e), r);
+    });
+    const bool last = in.now.flags & kLast;
+    in.close();
+    if (last) return true;
+    if (!in.open()) return false;
+  }
+}
+
+template <typename T, bool WHOLE, bool DROP>
+__global__ void __launch_bounds__(kBlock, 1) norm_forward_stream(NormArgs p) {
+  extern __shared__ __align__(128) unsigned char smem[];
+  auto& sh = *reinterpret_cast<ForwardShared<T, WHOLE>*>(smem);
+  drop_keep_stream(p.drop);
+  ring_init(sh.ring);
+  if (threadIdx.x >= kS) {
+    if (threadIdx.x == kS) {
+      const T* x = reinterpret_cast<const T*>(p.x);
+      produce<T, 1>(p, sh.ring, x, x);
+    }
+    return;
+  }
+  const Place at(p.C / (16 / (int)sizeof(T)), 0, kS);
+  Consumer<1, ForwardShared<T, WHOLE>::kStages> in(sh.ring);
+  while (in.open()) {
+    if (in.now.flags & kSecond ? !apply_unit<T, WHOLE, DROP>(p, at, in, sh.stats)
+                               : !stats_unit<T, WHOLE>(p, at, in, sh))
+      break;
+  }
+  if (!(in.now.flags & kEnd)) sh.ring.abort = 1;
+}
+
+// ---- backward ------------------------------------------------------------------------
+// RECT: a rectifier, whose side needs z to more than float32 (see norm_common.cuh).
+template <typename T, bool WHOLE>
+struct BackwardShared {
+  static constexpr int kV = 16 / sizeof(T), kStages = 4;
+  RingShared<2, kStages> ring;
+  float2 sums[kS * kV];  // sum dz, sum dz (x - mu)
+  float4 coef[1];        // [G] of the second pass's sample
+};
+
+// What z of a thread's channels takes, and dz in place of the output gradient.
+template <typename T, bool WHOLE, bool RECT, bool DROP>
+struct Slope {
+  static constexpr int V = 16 / sizeof(T), N = WHOLE ? 1 : V / 2, H = RECT ? V / 2 : 1;
+  float2 mu[N], a[V / 2], b[V / 2], al[H], bl[H];  // mu: minus mu
+  DropStream ds;
+  uint32_t keep = ~0u;
+
+  __device__ __forceinline__ Slope(const NormArgs& p, int sample, int c0) {
+    float m = 0.f, ml = 0.f, rh = 0.f, rl = 0.f;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      if (!WHOLE || v == 0) {
+        const double2 st = __ldg(p.stats + (long long)sample * p.G + (c0 + v) / p.Cg);
+        m = (float)st.x;
+        ml = (float)(st.x - (double)m);
+        rh = (float)st.y;
+        rl = (float)(st.y - (double)rh);
+        if (WHOLE) mu[0] = twice(-m);
+        else (v & 1 ? mu[v / 2 % N].y : mu[v / 2 % N].x) = -m;
+      }
+      const float w = param_f<T>(p.weight, p.param_f32, c0 + v, 1.f);
+      const float beta = param_f<T>(p.bias, p.param_f32, c0 + v, 0.f);
+      const float av = __fmul_rn(w, rh);  // no contraction: the pairs below need this rounding
+      float bv;
+      if (RECT) {
+        // a and b = beta - mu a as float pairs: products split by fma, sums by two-sum
+        const float alv = fmaf(w, rh, -av) + w * rl;
+        const float ph = __fmul_rn(-m, av), pl = -fmaf(m, av, ph);
+        bv = beta + ph;
+        const float z = bv - beta;
+        const float blv = ((beta - (bv - z)) + (ph - z)) + (pl - fmaf(m, alv, ml * av));
+        (v & 1 ? al[v / 2 % H].y : al[v / 2 % H].x) = alv;
+        (v & 1 ? bl[v / 2 % H].y : bl[v / 2 % H].x) = blv;
+      } else {
+        bv = fmaf(-ml, av, beta);  // for x - mu
+      }
+      (v & 1 ? a[v / 2].y : a[v / 2].x) = av;
+      (v & 1 ? b[v / 2].y : b[v / 2].x) = bv;
+    }
+    if (DROP) {
+      ds = drop_stream(p.drop);
+      if (p.drop.channel) keep = drop_keep<V>(ds, p.drop.threshold, (long long)sample * p.C + c0);
+    }
+  }
+
+  // g: output gradient -> dz; d: x -> x - mu
+  __device__ __forceinline__ void apply(const NormArgs& p, long long e, float2 (&d)[V / 2],
+                                        float2 (&g)[V / 2]) {
+    if (DROP) {
+      if (!p.drop.channel) keep = drop_keep<V>(ds, p.drop.threshold, e);
+#pragma unroll
+      for (int v = 0; v < V / 2; ++v) {
+        g[v] = mul2(g[v], twice(p.drop.factor));
+        keep2(g[v], keep >> (2 * v));
+      }
+    }
+    if (RECT) {
+      const float slope = p.act == LCB200_ACT_RELU ? 0.f : p.slope;
+#pragma unroll
+      for (int v = 0; v < V / 2; ++v) {
+        const float2 z =
+            add2(fma2(d[v], a[v], b[v]), fma2(d[v], al[v % H], bl[v % H]));
+        const float2 low = mul2(g[v], twice(slope));
+        g[v].x = z.x > 0.f ? g[v].x : low.x;
+        g[v].y = z.y > 0.f ? g[v].y : low.y;
+        d[v] = add2(d[v], mu[WHOLE ? 0 : v % N]);
+      }
+    } else {
+#pragma unroll
+      for (int v = 0; v < V / 2; ++v) d[v] = add2(d[v], mu[WHOLE ? 0 : v % N]);
+      if (p.act == LCB200_ACT_SILU) {
+#pragma unroll
+        for (int v = 0; v < V / 2; ++v) {
+          const float2 z = fma2(d[v], a[v], b[v]);
+          const float sx = sigmoid(z.x), sy = sigmoid(z.y);
+          g[v].x *= sx * fmaf(z.x, 1.f - sx, 1.f);
+          g[v].y *= sy * fmaf(z.y, 1.f - sy, 1.f);
+        }
+      }
+    }
+  }
+};
+
+template <typename T, bool WHOLE, bool RECT, bool DROP, typename C>
+__device__ __forceinline__ bool grad_sums_unit(const NormArgs& p, const Place& at, C& in,
+                                               float2* sums, bool* started) {
+  constexpr int V = 16 / sizeof(T);
+  const int b = in.now.b, seg = in.now.seg, c0 = at.col * V;
+  Slope<T, WHOLE, RECT, DROP> f(p, b, c0);
+  float2 sa[V / 2], sx[V / 2];
+#pragma unroll
+  for (int v = 0; v < V / 2; ++v) sa[v] = sx[v] = twice(0.f);
+  for (;;) {
+    const uint4 *xd = in.map(0), *gd = in.map(1);
+    const long long first = in.now.off + c0;
+    stage_rows<kVecs<2>>(at, in.now.rows, [&](int i, int row) {
+      float2 d[V / 2], g[V / 2];
+      Vec2<T>::unpack(xd[i], d);
+      Vec2<T>::unpack(gd[i], g);
+      f.apply(p, first + (long long)row * p.C, d, g);
+#pragma unroll
+      for (int v = 0; v < V / 2; ++v) {
+        sa[v] = add2(sa[v], g[v]);
+        sx[v] = fma2(g[v], d[v], sx[v]);
+      }
+    });
+    const bool last = in.now.flags & kLast;
+    in.close();
+    if (last) break;
+    if (!in.open()) return false;
+  }
+#pragma unroll
+  for (int v = 0; v < V / 2; ++v)
+    reinterpret_cast<float4*>(sums)[threadIdx.x * V / 2 + v] =
+        make_float4(sa[v].x, sx[v].x, sa[v].y, sx[v].y);
+  stream_sync();
+  // Channel sums in place, those of the parameters' gradients into the CTA's own row:
+  // X = r sum dz (x - mu), the sums centred on mu rounded to float32.
+  const double2* stats = p.stats + (long long)b * p.G;
+  const bool params = p.dweight || p.dbias;
+  for (int c = threadIdx.x; c < p.C; c += kS) {
+    float2 v = sums[c];
+    for (int r = 1; r < at.rp; ++r) {
+      const float2 e = sums[r * p.C + c];
+      v.x += e.x;
+      v.y += e.y;
+    }
+    sums[c] = v;
+    if (params) {
+      const double2 st = __ldg(stats + c / p.Cg);
+      double2* row = p.sums + (long long)blockIdx.x * p.C + c;
+      double2 t = *started ? *row : make_double2(0.0, 0.0);
+      t.x += v.x;
+      t.y += st.y * ((double)v.y - (st.x - (double)(float)st.x) * v.x);
+      *row = t;
+    }
+  }
+  *started = true;
+  stream_sync();
+  if (p.out) {
+    const int width = min(32, max(1, pow2_below(min(p.Cg, kS / min(p.G, kS)))));
+    const int lane = threadIdx.x % width;
+    for (int g0 = 0; g0 < p.G; g0 += kS / width) {
+      const int g = g0 + threadIdx.x / width;
+      double2 t = make_double2(0.0, 0.0);
+      if (g < p.G) {
+        for (int i = lane; i < p.Cg; i += width) {
+          const int c = g * p.Cg + i;
+          const double w = param_f<T>(p.weight, p.param_f32, c, 1.f);
+          const float2 e = sums[c];
+          t.x += w * e.x;
+          t.y += w * e.y;
+        }
+      }
+      t = lanes_sum(t, width);
+      if (g < p.G && lane == 0) put(p.part + (long long)seg * p.G + g, entry_of(t));
+    }
+    stream_sync();  // the sums have been read
+  }
+  return true;
+}
+
+template <typename T, bool WHOLE, bool RECT, bool DROP, typename C>
+__device__ __forceinline__ bool grad_input_unit(const NormArgs& p, const Place& at, C& in,
+                                                float4* coef) {
+  constexpr int V = 16 / sizeof(T), N = WHOLE ? 1 : V / 2;
+  const int b = in.now.b, c0 = at.col * V;
+  stream_sync();  // the last sample's have been read
+  sample_sums(p, b, &in.r.abort, [&](int g, double2 t) {
+    coef[g] = finish_coef(p, __ldg(p.stats + (long long)b * p.G + g), t);
+  });
+  stream_sync();
+  Slope<T, WHOLE, RECT, DROP> f(p, b, c0);
+  float2 k2[N], k3[N];
+#pragma unroll
+  for (int v = 0; v < 2 * N; ++v) {
+    const float4 k = coef[(c0 + (WHOLE ? 0 : v)) / p.Cg];
+    (v & 1 ? k2[v / 2].y : k2[v / 2].x) = k.y;
+    (v & 1 ? k3[v / 2].y : k3[v / 2].x) = k.z;
+  }
+  T* dst = reinterpret_cast<T*>(p.out);
+  for (;;) {
+    const uint4 *xd = in.map(0), *gd = in.map(1);
+    const long long first = in.now.off + c0;
+    stage_rows<kVecs<2>>(at, in.now.rows, [&](int i, int row) {
+      float2 d[V / 2], g[V / 2];
+      Vec2<T>::unpack(xd[i], d);
+      Vec2<T>::unpack(gd[i], g);
+      const long long e = first + (long long)row * p.C;
+      f.apply(p, e, d, g);
+#pragma unroll
+      for (int v = 0; v < V / 2; ++v)
+        g[v] = fma2(f.a[v], g[v], fma2(k2[WHOLE ? 0 : v % N], d[v], k3[WHOLE ? 0 : v % N]));
+      __stcs(reinterpret_cast<uint4*>(dst + e), Vec2<T>::pack(g));
+    });
+    const bool last = in.now.flags & kLast;
+    in.close();
+    if (last) return true;
+    if (!in.open()) return false;
+  }
+}
+
+template <typename T, bool WHOLE, bool RECT, bool DROP>
+__global__ void __launch_bounds__(kBlock, 1) norm_backward_stream(NormArgs p) {
+  extern __shared__ __align__(128) unsigned char smem[];
+  auto& sh = *reinterpret_cast<BackwardShared<T, WHOLE>*>(smem);
+  ring_init(sh.ring);
+  if (threadIdx.x >= kS) {
+    if (threadIdx.x == kS)
+      produce<T, 2>(p, sh.ring, reinterpret_cast<const T*>(p.x),
+                    reinterpret_cast<const T*>(p.dy));
+    return;
+  }
+  const Place at(p.C / (16 / (int)sizeof(T)), 0, kS);
+  Consumer<2, BackwardShared<T, WHOLE>::kStages> in(sh.ring);
+  bool started = false;
+  while (in.open()) {
+    if (in.now.flags & kSecond
+            ? !grad_input_unit<T, WHOLE, RECT, DROP>(p, at, in, sh.coef)
+            : !grad_sums_unit<T, WHOLE, RECT, DROP>(p, at, in, sh.sums, &started))
+      break;
+  }
+  if (!(in.now.flags & kEnd)) sh.ring.abort = 1;
+}
+
+// Weight and bias gradients from the CTAs' channel sums [CTAs, C]: two channels a CTA
+// (a 32-byte sector a row), rows over its threads, a fixed order throughout.
+constexpr int kParamChannels = 2;
+template <typename T>
+__global__ void __launch_bounds__(kS) norm_params_kernel(NormArgs p) {
+  __shared__ double2 sm[kS];
+  constexpr int kRows = kS / kParamChannels;
+  const int k = threadIdx.x % kParamChannels, c = blockIdx.x * kParamChannels + k;
+  double2 v = make_double2(0.0, 0.0);
+  if (c < p.C) {
+#pragma unroll 4
+    for (int i = threadIdx.x / kParamChannels; i < p.ctas; i += kRows) {
+      const double2 e = __ldg(p.sums + (long long)i * p.C + c);
+      v.x += e.x;
+      v.y += e.y;
+    }
+  }
+  sm[threadIdx.x] = v;
+  for (int o = kS / 2; o >= kParamChannels; o /= 2) {
+    __syncthreads();
+    if (threadIdx.x < o) {
+      sm[threadIdx.x].x += sm[threadIdx.x + o].x;
+      sm[threadIdx.x].y += sm[threadIdx.x + o].y;
+    }
+  }
+  if (threadIdx.x < kParamChannels && c < p.C) {
+    put_param<T>(p.dbias, p.param_f32, c, sm[threadIdx.x].x);
+    put_param<T>(p.dweight, p.param_f32, c, sm[threadIdx.x].y);
+  }
+}
+
+// ---- host ----------------------------------------------------------------------------
+template <typename K>
+bool launch_kernel(K kernel, size_t smem, const NormArgs& p, const char* what, cudaStream_t s) {
+  // the static shared memory counts towards the 48 KB that need no opt-in
+  if (!ensure_smem_attr((const void*)kernel, smem + 1024)) return false;
+  NormArgs args = p;
+  void* argv[] = {&args};
+  if (cudaLaunchCooperativeKernel((const void*)kernel, dim3(p.ctas), dim3(kBlock), argv, smem,
+                                  s) != cudaSuccess)
+    return check_launch(what);
+  count_launch();
+  return check_launch(what);
+}
+
+template <typename T, bool WHOLE, bool DROP>
+bool launch_w(const NormArgs& p, bool backward, cudaStream_t s) {
+  if (!backward)
+    return launch_kernel(norm_forward_stream<T, WHOLE, DROP>,
+                         sizeof(ForwardShared<T, WHOLE>) + sizeof(double2) * p.G, p, "group norm",
+                         s);
+  const size_t smem = sizeof(BackwardShared<T, WHOLE>) + sizeof(float4) * p.G;
+  const bool rect = p.act == LCB200_ACT_RELU || p.act == LCB200_ACT_LEAKY_RELU;
+  if (!(rect ? launch_kernel(norm_backward_stream<T, WHOLE, true, DROP>, smem, p,
+                             "group norm backward", s)
+             : launch_kernel(norm_backward_stream<T, WHOLE, false, DROP>, smem, p,
+                             "group norm backward", s)))
+    return false;
+  if (!p.dweight && !p.dbias) return true;
+  norm_params_kernel<T><<<(p.C + kParamChannels - 1) / kParamChannels, kS, 0, s>>>(p);
+  count_launch();
+  return check_launch("group norm parameter gradients");
+}
+
+template <typename T>
+bool launch_t(const NormArgs& p, bool backward, cudaStream_t s) {
+  const bool drop = p.drop.threshold != 0;
+  if (p.Cg % (16 / sizeof(T)) == 0)
+    return drop ? launch_w<T, true, true>(p, backward, s) : launch_w<T, true, false>(p, backward, s);
+  return drop ? launch_w<T, false, true>(p, backward, s) : launch_w<T, false, false>(p, backward, s);
+}
+
+}  // namespace
+
+bool stream_norm(const NormArgs& p, int dtype, bool backward, cudaStream_t s) {
+  if (dtype == LCB200_F32) return launch_t<float>(p, backward, s);
+  if (dtype == LCB200_F16) return launch_t<__half>(p, backward, s);
+  return launch_t<__nv_bfloat16>(p, backward, s);
+}
+
+int stream_stage_rows(int C, int dtype, bool backward) {
+  const int cols = std::max(1, C / (16 / (int)dtype_bytes(dtype)));
+  return (backward ? kVecs<2> : kVecs<1>) * std::max(1, kS / cols);
+}
+
+int stream_norm_status(bool reset) { return read_norm_status(reset); }
+
+}  // namespace lcb200
