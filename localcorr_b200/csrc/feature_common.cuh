@@ -71,14 +71,24 @@ struct DropArgs {
   long long* rng_used;     // device, receives {seed, offset}; may be null
 };
 
+// The key schedule is kept (20 registers): the integer pipes are what a 16-bit map's
+// draws use most of.
 struct DropStream {
-  uint32_t k0, k1, c2, c3;
+  uint32_t k0[10], k1[10], c2, c3;
 };
 
 __device__ __forceinline__ DropStream drop_stream(const DropArgs& d) {
   const unsigned long long seed = d.rng ? __ldg(d.rng) : d.seed;
   const unsigned long long off = d.rng ? __ldg(d.rng + 1) : d.offset;
-  return DropStream{(uint32_t)seed, (uint32_t)(seed >> 32), (uint32_t)off, (uint32_t)(off >> 32)};
+  DropStream s;
+#pragma unroll
+  for (uint32_t r = 0; r < 10; ++r) {
+    s.k0[r] = (uint32_t)seed + r * 0x9E3779B9u;
+    s.k1[r] = (uint32_t)(seed >> 32) + r * 0xBB67AE85u;
+  }
+  s.c2 = (uint32_t)off;
+  s.c3 = (uint32_t)(off >> 32);
+  return s;
 }
 
 // Leaves the stream that a forward call used for its backward pass: the caller
@@ -92,17 +102,14 @@ __device__ __forceinline__ void drop_keep_stream(const DropArgs& d) {
 
 __device__ __forceinline__ uint4 drop_block(const DropStream& s, unsigned long long i) {
   uint32_t c0 = (uint32_t)i, c1 = (uint32_t)(i >> 32), c2 = s.c2, c3 = s.c3;
-  uint32_t k0 = s.k0, k1 = s.k1;
 #pragma unroll
   for (int r = 0; r < 10; ++r) {
-    const uint32_t h0 = __umulhi(0xD2511F53u, c0), l0 = 0xD2511F53u * c0;
-    const uint32_t h1 = __umulhi(0xCD9E8D57u, c2), l1 = 0xCD9E8D57u * c2;
-    c0 = h1 ^ c1 ^ k0;
-    c1 = l1;
-    c2 = h0 ^ c3 ^ k1;
-    c3 = l0;
-    k0 += 0x9E3779B9u;
-    k1 += 0xBB67AE85u;
+    const unsigned long long p0 = (unsigned long long)0xD2511F53u * c0;
+    const unsigned long long p1 = (unsigned long long)0xCD9E8D57u * c2;
+    c0 = (uint32_t)(p1 >> 32) ^ c1 ^ s.k0[r];
+    c1 = (uint32_t)p1;
+    c2 = (uint32_t)(p0 >> 32) ^ c3 ^ s.k1[r];
+    c3 = (uint32_t)p0;
   }
   return make_uint4(c0, c1, c2, c3);
 }
@@ -110,6 +117,12 @@ __device__ __forceinline__ uint4 drop_block(const DropStream& s, unsigned long l
 __device__ __forceinline__ uint32_t drop_piece(const uint4& w, int e) {
   const uint32_t word = e < 4 ? (e < 2 ? w.x : w.y) : (e < 6 ? w.z : w.w);
   return (e & 1) ? word >> 16 : word & 0xffffu;
+}
+
+// All ones in the halves of word w whose draws stay: the sign of draw - threshold,
+// spread over a half.
+__device__ __forceinline__ uint32_t drop_mask2(uint32_t w, uint32_t threshold) {
+  return ~__byte_perm((w & 0xffffu) - threshold, (w >> 16) - threshold, 0xffbb);
 }
 
 // Bit v: element e0 + v stays. V divides 8 and e0 is a multiple of V.

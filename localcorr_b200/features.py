@@ -15,36 +15,29 @@ are ``torch.ops.localcorr.group_norm`` / ``.dropout`` (torch_ops.py).
 
 from __future__ import annotations
 
+import contextlib
 import functools
 
 import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .ops import _require_cuda, _stream, _timed
+from .ops import _require_cuda, _timed
 
 _DTYPES = {torch.float32: _lib.F32, torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
 _MODES = ("element", "channel")
 
 
-class _on_device:
+_HERE = contextlib.nullcontext()
+
+
+def _on_device(index):
     """``torch.cuda.device`` that costs nothing when the device is current."""
-
-    def __new__(cls, t):
-        if t.device.index == torch.cuda.current_device():
-            return _HERE
-        return torch.cuda.device(t.device)
+    return _HERE if index == torch.cuda.current_device() else torch.cuda.device(index)
 
 
-class _Here:
-    def __enter__(self):
-        return self
-
-    def __exit__(self, *exc):
-        return False
-
-
-_HERE = _Here()
+def _stream(index):
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
 # ---------------------------------------------------------------------------
@@ -144,11 +137,12 @@ def dropout_forward(x, residual, p, channel, rng, seed, offset):
     b, rows, c = _rows(x)
     y = torch.empty_like(x)
     used = torch.empty(2, dtype=torch.int64, device=x.device)
-    nbytes = x.numel() * x.element_size() * (3 if residual is not None else 2)
-    with _on_device(x):
+    dev = x.get_device()
+    with _on_device(dev):
         ok = _timed("dropout", lambda: lib.launchLocalCorrB200Dropout(
             x.data_ptr(), _ptr(residual), y.data_ptr(), b, rows, c, _DTYPES[x.dtype], p, channel,
-            seed, offset, _ptr(rng), used.data_ptr(), _stream(x)), nbytes)
+            seed, offset, _ptr(rng), used.data_ptr(), _stream(dev)),
+            x.nbytes * (3 if residual is not None else 2))
     _lib.check(ok, "dropout", lib)
     return y, used
 
@@ -159,10 +153,11 @@ def dropout_backward(grad, used, p, channel):
     grad = grad.contiguous()
     b, rows, c = _rows(grad)
     gx = torch.empty_like(grad)
-    with _on_device(grad):
+    dev = grad.get_device()
+    with _on_device(dev):
         ok = _timed("dropout", lambda: lib.launchLocalCorrB200Dropout(
             grad.data_ptr(), None, gx.data_ptr(), b, rows, c, _DTYPES[grad.dtype], p, channel, 0,
-            0, used.data_ptr(), None, _stream(grad)), 2 * grad.numel() * grad.element_size())
+            0, used.data_ptr(), None, _stream(dev)), 2 * grad.nbytes)
     _lib.check(ok, "dropout backward", lib)
     return gx
 
@@ -175,7 +170,7 @@ def _norm_workspace_bytes(device, b, rows, c, groups, dtype, backward):
 
 
 def _norm_workspace(x, b, rows, c, groups, backward):
-    n = _norm_workspace_bytes(x.device.index, b, rows, c, groups, x.dtype, backward)
+    n = _norm_workspace_bytes(x.get_device(), b, rows, c, groups, x.dtype, backward)
     return torch.empty(n, dtype=torch.uint8, device=x.device)
 
 
@@ -186,7 +181,7 @@ def _params_f32(x, weight, bias):
 
 def group_norm_forward(x, weight, bias, num_groups, eps, activation, negative_slope, p, channel,
                        rng, seed, offset):
-    """(y, statistics float64 [B, G, 2], the stream used: [2] with p > 0, else [0])."""
+    """(y, statistics float64 [B, G, 2], the stream used: int64 [2], None with p = 0)."""
     lib = _lib.require_library()
     x = x.contiguous()
     weight = weight.contiguous() if weight is not None else None
@@ -196,15 +191,15 @@ def group_norm_forward(x, weight, bias, num_groups, eps, activation, negative_sl
     b, rows, c = _rows(x)
     y = torch.empty_like(x)
     stats = torch.empty((b, num_groups, 2), dtype=torch.float64, device=x.device)
-    used = torch.empty(2 if p > 0 else 0, dtype=torch.int64, device=x.device)
+    used = torch.empty(2, dtype=torch.int64, device=x.device) if p > 0 else None
     ws = _norm_workspace(x, b, rows, c, num_groups, False)
-    with _on_device(x):
+    dev = x.get_device()
+    with _on_device(dev):
         ok = _timed("group_norm_fwd", lambda: lib.launchLocalCorrB200GroupNormForward(
             x.data_ptr(), _ptr(weight), _ptr(bias), y.data_ptr(), stats.data_ptr(), b, rows, c,
             num_groups, _DTYPES[x.dtype], _params_f32(x, weight, bias), eps,
             _lib.ACT_CODES[activation], negative_slope, p, channel, seed, offset, _ptr(rng),
-            used.data_ptr() if p > 0 else None, ws.data_ptr(), ws.numel(), _stream(x)),
-            2 * x.numel() * x.element_size())
+            _ptr(used), ws.data_ptr(), ws.numel(), _stream(dev)), 2 * x.nbytes)
     _lib.check(ok, "group norm", lib)
     return y, stats, used
 
@@ -224,13 +219,13 @@ def group_norm_backward(grad_y, x, weight, bias, stats, used, num_groups, activa
     gw = torch.empty_like(weight) if need_weight and weight is not None else None
     gb = torch.empty_like(bias) if need_bias and bias is not None else None
     ws = _norm_workspace(x, b, rows, c, num_groups, True)
-    with _on_device(x):
+    dev = x.get_device()
+    with _on_device(dev):
         ok = _timed("group_norm_bwd", lambda: lib.launchLocalCorrB200GroupNormBackward(
             grad_y.data_ptr(), x.data_ptr(), _ptr(weight), _ptr(bias), stats.data_ptr(),
             _ptr(gx), _ptr(gw), _ptr(gb), b, rows, c, num_groups, _DTYPES[x.dtype],
             _params_f32(x, weight, bias), _lib.ACT_CODES[activation], negative_slope, p, channel,
-            0, 0, used.data_ptr() if p > 0 else None, ws.data_ptr(), ws.numel(), _stream(x)),
-            3 * x.numel() * x.element_size())
+            0, 0, _ptr(used), ws.data_ptr(), ws.numel(), _stream(dev)), 3 * x.nbytes)
     _lib.check(ok, "group norm backward", lib)
     return gx, gw, gb
 

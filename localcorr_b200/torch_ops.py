@@ -243,8 +243,9 @@ spatial_corr.register_autograd(_sc_backward, setup_context=_sc_setup)
 def group_norm(x: Tensor, weight: Optional[Tensor], bias: Optional[Tensor], num_groups: int,
                eps: float, activation: str, negative_slope: float, p: float, channel: bool,
                rng: Optional[Tensor], seed: int, offset: int) -> tuple[Tensor, Tensor, Tensor]:
-    return features.group_norm_forward(x, weight, bias, num_groups, eps, activation,
-                                       negative_slope, p, channel, rng, seed, offset)
+    y, stats, used = features.group_norm_forward(x, weight, bias, num_groups, eps, activation,
+                                                 negative_slope, p, channel, rng, seed, offset)
+    return y, stats, used if used is not None else x.new_empty((0,), dtype=torch.int64)
 
 
 @group_norm.register_fake
@@ -260,7 +261,7 @@ def _absent(like: Tensor) -> Tensor:
 
 @custom_op(f"{_NS}::group_norm_backward", mutates_args=(), device_types="cuda")
 def group_norm_backward(grad_y: Tensor, x: Tensor, weight: Optional[Tensor],
-                        bias: Optional[Tensor], stats: Tensor, used: Tensor, num_groups: int,
+                        bias: Optional[Tensor], stats: Tensor, used: Optional[Tensor], num_groups: int,
                         activation: str, negative_slope: float, p: float,
                         channel: bool) -> tuple[Tensor, Tensor, Tensor]:
     """Gradients of x, weight and bias (empty for an absent parameter)."""
