@@ -365,12 +365,85 @@ __global__ void __launch_bounds__(kT, kOcc) norm_backward_kernel(NormArgs p) {
   });
 }
 
+// ---- whole samples ------------------------------------------------------------------------
+// A CTA makes both passes of a sample: nothing to exchange, one ordinary launch, the
+// second read out of L1 and L2. For samples too small to divide and for many small ones.
+template <typename T, int V, bool DROP>
+__global__ void __launch_bounds__(kT, kOcc) norm_forward_samples(NormArgs p) {
+  __shared__ double2 sm[kT * V];
+  drop_keep_stream(p.drop);
+  for (int b = blockIdx.x; b < p.B; b += gridDim.x) {
+    stats_slice<T, V>(p, b, 0, sm);
+    for (int g = threadIdx.x; g < p.G; g += kT) {
+      const long long i = (long long)b * p.G + g;
+      p.stats[i] = finish_stats(p, __ldcg(p.part + i));
+    }
+    cta_sync();
+    apply_slice<T, V, DROP>(p, b, 0);
+  }
+}
+
+template <typename T, int V, bool DROP>
+__global__ void __launch_bounds__(kT, kOcc) norm_backward_samples(NormArgs p) {
+  __shared__ __align__(16) float2 sm[kT * (V < 2 ? 2 : V)];  // also kT double2 sums
+  double2* smd = reinterpret_cast<double2*>(sm);
+  for (int b = blockIdx.x; b < p.B; b += gridDim.x) {
+    grad_sums_slice<T, V, DROP>(p, b, 0, sm);
+    for (int c = threadIdx.x; c < p.C; c += kT)
+      finish_channel(p, b, c, as_double2(__ldcg(p.bpart + (long long)b * p.C + c)));
+    finish_coef<T>(p, b);
+    cta_sync();
+    if (p.out) grad_input_slice<T, V, DROP>(p, b, 0);
+  }
+  if (p.B == 1) param_grads<T>(p, smd);
+}
+
+// Weight and bias gradients from per-sample or per-CTA channel sums [n, C]: two channels
+// a CTA (a 32-byte sector a row), rows over its threads, a fixed order throughout.
+constexpr int kParamChannels = 2;
+template <typename T>
+__global__ void __launch_bounds__(kT) norm_params_kernel(NormArgs p, int n) {
+  __shared__ double2 sm[kT];
+  constexpr int kRows = kT / kParamChannels;
+  const int k = threadIdx.x % kParamChannels, c = blockIdx.x * kParamChannels + k;
+  double2 v = make_double2(0.0, 0.0);
+  if (c < p.C) {
+#pragma unroll 4
+    for (int i = threadIdx.x / kParamChannels; i < n; i += kRows) {
+      const double2 e = __ldg(p.sums + (long long)i * p.C + c);
+      v.x += e.x;
+      v.y += e.y;
+    }
+  }
+  sm[threadIdx.x] = v;
+  for (int o = kT / 2; o >= kParamChannels; o /= 2) {
+    __syncthreads();
+    if (threadIdx.x < o) {
+      sm[threadIdx.x].x += sm[threadIdx.x + o].x;
+      sm[threadIdx.x].y += sm[threadIdx.x + o].y;
+    }
+  }
+  if (threadIdx.x < kParamChannels && c < p.C) {
+    put_param<T>(p.dbias, p.param_f32, c, sm[threadIdx.x].x);
+    put_param<T>(p.dweight, p.param_f32, c, sm[threadIdx.x].y);
+  }
+}
+
+template <typename T>
+bool launch_params(const NormArgs& p, int n, cudaStream_t s) {
+  if (!p.dweight && !p.dbias) return true;
+  norm_params_kernel<T><<<(p.C + kParamChannels - 1) / kParamChannels, kT, 0, s>>>(p, n);
+  count_launch();
+  return check_launch("group norm parameter gradients");
+}
+
 // ---- host ---------------------------------------------------------------------------------
 // Widest rows of the streamed kernels: their per-group values, a double2 or float4
 // each, share a CTA's memory with the ring.
 constexpr int kStreamChannels = 2048;
 
 struct Plan {
+  bool samples;  // whole samples
   int slices, fan, sets;
   long long slice_rows;
   uint32_t units, lag;
@@ -389,6 +462,13 @@ Plan make_plan(int B, long long S, int C, int dtype, bool backward) {
   const long long step = 4 * rp, slots = (long long)device_sms() * kOcc;
   const long long n = (long long)std::min<double>(4, (double)S * B / (double)(2 * slots * step));
   q.slice_rows = std::min<long long>(S, std::max<long long>(1, n) * step);
+  // whole samples where one CTA's two passes cost less than the exchange between CTAs.
+  // Measured with C = 256 float16, 1 and 300 samples, whole against divided: forward
+  // 64 KB a sample 8.6 and 14.7 us against 12.4 and 26.4, 256 KB 18.9 and 47.7 against
+  // 10.3 and 45.7; backward 8 KB 9.6 and 17.5 against 15.4 and 30.1, 32 KB 14.4 against
+  // 16.5, 64 KB 21.4 and 39.2 against 14.4 and 42.4
+  q.samples = (double)S * C * es <= (backward ? 32 : 128) * 1024;
+  if (q.samples) q.slice_rows = S;
   const long long slices = (S + q.slice_rows - 1) / q.slice_rows, units = slices * B;
   q.slices = (int)slices;
   q.units = (uint32_t)units;
@@ -428,7 +508,7 @@ Layout layout(const Plan& q, int B, int C, int G, bool backward) {
   };
   Layout l{};
   take(l.flags = sizeof(uint32_t) * (2 + (2 + (size_t)q.sets) * B));
-  l.part = take(sizeof(double2) * (size_t)G * std::max<size_t>(q.units, q.slots));
+  l.part = take(sizeof(double2) * (size_t)G * std::max<size_t>(q.units, q.samples ? 0 : q.slots));
   l.plain = at;
   l.set_part = take(sizeof(double2) * (size_t)(backward ? C : G) * B * q.sets);
   if (backward) {
@@ -441,34 +521,42 @@ Layout layout(const Plan& q, int B, int C, int G, bool backward) {
 }
 
 template <typename T, int V, bool DROP>
-bool launch_kernel(const NormArgs& p, bool backward, cudaStream_t s) {
-  const unsigned grid = std::min<unsigned>(p.tickets, (unsigned)(device_sms() * kOcc));
-  if (backward) norm_backward_kernel<T, V, DROP><<<grid, kT, 0, s>>>(p);
-  else norm_forward_kernel<T, V, DROP><<<grid, kT, 0, s>>>(p);
+bool launch_kernel(const NormArgs& p, bool backward, bool samples, cudaStream_t s) {
+  const unsigned slots = (unsigned)(device_sms() * kOcc);
+  if (samples) {
+    const unsigned grid = std::min<unsigned>((unsigned)p.B, slots);
+    if (backward) norm_backward_samples<T, V, DROP><<<grid, kT, 0, s>>>(p);
+    else norm_forward_samples<T, V, DROP><<<grid, kT, 0, s>>>(p);
+  } else {
+    const unsigned grid = std::min<unsigned>(p.tickets, slots);
+    if (backward) norm_backward_kernel<T, V, DROP><<<grid, kT, 0, s>>>(p);
+    else norm_forward_kernel<T, V, DROP><<<grid, kT, 0, s>>>(p);
+  }
   count_launch();
-  return check_launch(backward ? "group norm backward" : "group norm");
+  if (!check_launch(backward ? "group norm backward" : "group norm")) return false;
+  return !(samples && backward && p.B > 1) || launch_params<T>(p, p.B, s);
 }
 
 template <typename T, int V>
-bool launch_v(const NormArgs& p, bool backward, cudaStream_t s) {
-  return p.drop.threshold != 0 ? launch_kernel<T, V, true>(p, backward, s)
-                               : launch_kernel<T, V, false>(p, backward, s);
+bool launch_v(const NormArgs& p, bool backward, bool samples, cudaStream_t s) {
+  return p.drop.threshold != 0 ? launch_kernel<T, V, true>(p, backward, samples, s)
+                               : launch_kernel<T, V, false>(p, backward, samples, s);
 }
 
 template <typename T>
-bool launch_t(const NormArgs& p, int dtype, bool backward, cudaStream_t s) {
+bool launch_t(const NormArgs& p, int dtype, bool backward, bool samples, cudaStream_t s) {
   switch (vec_width(dtype, p.C, p.x, p.out, p.dy)) {
-    case 8: return launch_v<T, (sizeof(T) == 2 ? 8 : 4)>(p, backward, s);
-    case 4: return launch_v<T, 4>(p, backward, s);
-    case 2: return launch_v<T, 2>(p, backward, s);
-    default: return launch_v<T, 1>(p, backward, s);
+    case 8: return launch_v<T, (sizeof(T) == 2 ? 8 : 4)>(p, backward, samples, s);
+    case 4: return launch_v<T, 4>(p, backward, samples, s);
+    case 2: return launch_v<T, 2>(p, backward, samples, s);
+    default: return launch_v<T, 1>(p, backward, samples, s);
   }
 }
 
-bool launch(const NormArgs& p, int dtype, bool backward, cudaStream_t s) {
-  if (dtype == LCB200_F32) return launch_t<float>(p, dtype, backward, s);
-  if (dtype == LCB200_F16) return launch_t<__half>(p, dtype, backward, s);
-  return launch_t<__nv_bfloat16>(p, dtype, backward, s);
+bool launch(const NormArgs& p, int dtype, bool backward, bool samples, cudaStream_t s) {
+  if (dtype == LCB200_F32) return launch_t<float>(p, dtype, backward, samples, s);
+  if (dtype == LCB200_F16) return launch_t<__half>(p, dtype, backward, samples, s);
+  return launch_t<__nv_bfloat16>(p, dtype, backward, samples, s);
 }
 
 }  // namespace
@@ -523,7 +611,7 @@ bool feature_norm(const void* x, const void* dy, const void* weight, const void*
   p.chunks = q.chunks;
   p.tickets = out ? 2 * q.units : q.units;
   const int full = 16 / (int)dtype_bytes(dtype);
-  const bool stream = C <= kStreamChannels && vec_width(dtype, C, x, out, dy) == full;
+  const bool stream = !q.samples && C <= kStreamChannels && vec_width(dtype, C, x, out, dy) == full;
   p.ticket = reinterpret_cast<uint32_t*>(w);
   p.done = p.ticket + 2;
   p.sets_done = p.done + (size_t)B * q.sets;
@@ -536,10 +624,16 @@ bool feature_norm(const void* x, const void* dy, const void* weight, const void*
   p.dweight = dweight;
   p.dbias = dbias;
   p.drop = drop;
-  if ((stream ? cudaMemsetAsync(w + l.part, 0xff, sizeof(double2) * (size_t)G * q.slots, s)
+  if (!q.samples &&
+      (stream ? cudaMemsetAsync(w + l.part, 0xff, sizeof(double2) * (size_t)G * q.slots, s)
               : cudaMemsetAsync(w, 0, l.flags, s)) != cudaSuccess)
     return check_launch("group norm: memset of the counters");
-  return stream ? stream_norm(p, dtype, backward, s) : launch(p, dtype, backward, s);
+  if (!stream) return launch(p, dtype, backward, q.samples, s);
+  if (!stream_norm(p, dtype, backward, s)) return false;
+  if (!backward) return true;
+  if (dtype == LCB200_F32) return launch_params<float>(p, p.ctas, s);
+  if (dtype == LCB200_F16) return launch_params<__half>(p, p.ctas, s);
+  return launch_params<__nv_bfloat16>(p, p.ctas, s);
 }
 
 int feature_device_status(bool reset) {

@@ -814,37 +814,6 @@ __global__ void __launch_bounds__(kBlock, 1) norm_backward_stream(NormArgs p) {
   if (!(in.now.flags & kEnd)) sh.ring.abort = 1;
 }
 
-// Weight and bias gradients from the CTAs' channel sums [CTAs, C]: two channels a CTA
-// (a 32-byte sector a row), rows over its threads, a fixed order throughout.
-constexpr int kParamChannels = 2;
-template <typename T>
-__global__ void __launch_bounds__(kS) norm_params_kernel(NormArgs p) {
-  __shared__ double2 sm[kS];
-  constexpr int kRows = kS / kParamChannels;
-  const int k = threadIdx.x % kParamChannels, c = blockIdx.x * kParamChannels + k;
-  double2 v = make_double2(0.0, 0.0);
-  if (c < p.C) {
-#pragma unroll 4
-    for (int i = threadIdx.x / kParamChannels; i < p.ctas; i += kRows) {
-      const double2 e = __ldg(p.sums + (long long)i * p.C + c);
-      v.x += e.x;
-      v.y += e.y;
-    }
-  }
-  sm[threadIdx.x] = v;
-  for (int o = kS / 2; o >= kParamChannels; o /= 2) {
-    __syncthreads();
-    if (threadIdx.x < o) {
-      sm[threadIdx.x].x += sm[threadIdx.x + o].x;
-      sm[threadIdx.x].y += sm[threadIdx.x + o].y;
-    }
-  }
-  if (threadIdx.x < kParamChannels && c < p.C) {
-    put_param<T>(p.dbias, p.param_f32, c, sm[threadIdx.x].x);
-    put_param<T>(p.dweight, p.param_f32, c, sm[threadIdx.x].y);
-  }
-}
-
 // ---- host ----------------------------------------------------------------------------
 template <typename K>
 bool launch_kernel(K kernel, size_t smem, const NormArgs& p, const char* what, cudaStream_t s) {
@@ -867,15 +836,10 @@ bool launch_w(const NormArgs& p, bool backward, cudaStream_t s) {
                          s);
   const size_t smem = sizeof(BackwardShared<T, WHOLE>) + sizeof(float4) * p.G;
   const bool rect = p.act == LCB200_ACT_RELU || p.act == LCB200_ACT_LEAKY_RELU;
-  if (!(rect ? launch_kernel(norm_backward_stream<T, WHOLE, true, DROP>, smem, p,
-                             "group norm backward", s)
-             : launch_kernel(norm_backward_stream<T, WHOLE, false, DROP>, smem, p,
-                             "group norm backward", s)))
-    return false;
-  if (!p.dweight && !p.dbias) return true;
-  norm_params_kernel<T><<<(p.C + kParamChannels - 1) / kParamChannels, kS, 0, s>>>(p);
-  count_launch();
-  return check_launch("group norm parameter gradients");
+  return rect ? launch_kernel(norm_backward_stream<T, WHOLE, true, DROP>, smem, p,
+                              "group norm backward", s)
+              : launch_kernel(norm_backward_stream<T, WHOLE, false, DROP>, smem, p,
+                              "group norm backward", s);
 }
 
 template <typename T>
