@@ -1,12 +1,15 @@
-// Group norm: plan and launch, and the kernels for maps that the streamed ones
-// (norm_stream.cu) do not take: rows that are no whole number of aligned 16-byte
-// vectors, or wider than a CTA's threads.
+// Group norm: plan and launch, the kernels for whole samples, and the plain kernels for
+// maps that the streamed ones (norm_stream.cu) do not take: rows that are no whole
+// number of aligned 16-byte vectors, too wide, or of too many groups. The plain kernels
+// move 1 to 2.5 TB/s where the streamed ones move 3 to 4 (8 x 32400 x 99 float16
+// element by element: 92 us forward; x 96: 35 us).
 #include "norm_common.cuh"
 
 namespace lcb200 {
 
 bool stream_norm(const NormArgs& p, int dtype, bool backward, cudaStream_t s);
 int stream_norm_status(bool reset);
+int stream_ctas();  // resident CTAs
 int stream_stage_rows(int C, int dtype, bool backward);  // rows of a stage, at least 1
 
 namespace {
@@ -24,53 +27,35 @@ __device__ void stats_slice(const NormArgs& p, int b, int j, double2* sm) {
   for (int cb = 0; cb < cols; cb += kT) {
     const Place at(cols, cb);
     if (at.on) {
-      float s[V], q[V], k[V];
+      double s[V], q[V];
 #pragma unroll
-      for (int v = 0; v < V; ++v) s[v] = q[v] = k[v] = 0.f;
-      int n = 0;
+      for (int v = 0; v < V; ++v) s[v] = q[v] = 0.0;
       const T* ptr = xb + (long long)at.col * V;
-      long long r = r0 + at.row;
-      if (r < r1) {
-        Vec<T, V>::unpack(Vec<T, V>::load(ptr + r * p.C), k);
-        n = 1;
-        r += at.rp;
-      }
       const long long step = at.rp;
+      auto one = [&](typename Vec<T, V>::Raw raw) {
+        float f[V];
+        Vec<T, V>::unpack(raw, f);
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          const double x = f[v];
+          s[v] += x;
+          q[v] = fma(x, x, q[v]);
+        }
+      };
+      long long r = r0 + at.row;
       for (; r + (kUnroll - 1) * step < r1; r += kUnroll * step) {
         typename Vec<T, V>::Raw raw[kUnroll];
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u) raw[u] = Vec<T, V>::load(ptr + (r + u * step) * p.C);
 #pragma unroll
-        for (int u = 0; u < kUnroll; ++u) {
-          float f[V];
-          Vec<T, V>::unpack(raw[u], f);
-#pragma unroll
-          for (int v = 0; v < V; ++v) {
-            const float d = f[v] - k[v];
-            s[v] += d;
-            q[v] = fmaf(d, d, q[v]);
-          }
-        }
-        n += kUnroll;
+        for (int u = 0; u < kUnroll; ++u) one(raw[u]);
       }
-      for (; r < r1; r += step) {
-        float f[V];
-        Vec<T, V>::unpack(Vec<T, V>::load(ptr + r * p.C), f);
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-          const float d = f[v] - k[v];
-          s[v] += d;
-          q[v] = fmaf(d, d, q[v]);
-        }
-        ++n;
-      }
-      // sum x = s + n K, sum x^2 = q + 2 K s + n K^2, in float64
+      for (; r < r1; r += step) one(Vec<T, V>::load(ptr + r * p.C));
       double2 tot = make_double2(0.0, 0.0);
       double2* dst = sm + ((long long)at.row * at.nc + (at.col - cb)) * per;
 #pragma unroll
       for (int v = 0; v < V; ++v) {
-        const double kv = k[v], sv = s[v];
-        const double2 e = make_double2(sv + n * kv, (double)q[v] + kv * (2.0 * sv + n * kv));
+        const double2 e = make_double2(s[v], q[v]);
         if (whole) {
           tot.x += e.x;
           tot.y += e.y;
@@ -438,16 +423,20 @@ bool launch_params(const NormArgs& p, int n, cudaStream_t s) {
 }
 
 // ---- host ---------------------------------------------------------------------------------
-// Widest rows of the streamed kernels: their per-group values, a double2 or float4
-// each, share a CTA's memory with the ring.
-constexpr int kStreamChannels = 2048;
+// The streamed kernels take rows of whole 16-byte vectors, one a thread at most, and up
+// to 512 groups: their per-group values share a CTA's memory with the ring, and two
+// CTAs have to fit a multiprocessor.
+bool streams(int C, int G, int dtype, int width) {
+  const int full = 16 / (int)dtype_bytes(dtype);
+  return width == full && C / full <= kT && G <= 512;
+}
 
 struct Plan {
   bool samples;  // whole samples
   int slices, fan, sets;
   long long slice_rows;
   uint32_t units, lag;
-  int ctas, stage_rows, chunk, chunks;
+  int teams, ctas, stage_rows, chunk, chunks;
   long long slots;
   bool ok;
 };
@@ -474,18 +463,20 @@ Plan make_plan(int B, long long S, int C, int dtype, bool backward) {
   q.units = (uint32_t)units;
   q.lag = (uint32_t)std::min<long long>(
       units, slices + (long long)((32 << 20) / (maps * q.slice_rows * C * es)));
-  // streamed kernels: chunks of up to 160 MB. L2 holds less of that, but the exchange of
-  // a chunk's sums costs 5 to 6 us: 8 x 135 x 240 x 256 float16, forward and backward,
-  // takes 242 us in chunks of 40 MB, 223 of 72 and 201 of 200 MB
-  const double target = 160 << 20;
+  // streamed kernels: up to 16 MB one chunk for both teams together, else an even number
+  // of chunks of up to 160 MB. Smaller chunks would be read a second time out of L2
+  // altogether (33 MB: 141 of 133 MB from HBM, 66 MB: 183), but each exchange of sums
+  // costs more than that saves: 8 x 135 x 240 x 256 float16 takes forward 77, 71 and 71 us
+  // and backward 155, 132 and 120 us in chunks of at most 30, 72 and 160 MB
   const double total = maps * (double)S * B * C * es;
-  const long long k = std::min<long long>(B, (long long)(total / target) + 1);
+  const long long k = std::min<long long>(
+      B, total < (16 << 20) ? 1 : 2 * (long long)(total / (2.0 * (160 << 20))) + 2);
   q.chunk = (int)((B + k - 1) / k);
   q.chunks = (B + q.chunk - 1) / q.chunk;
+  q.teams = q.chunks > 1 ? 2 : 1;
   q.stage_rows = stream_stage_rows(C, dtype, backward);
-  q.ctas = device_sms();
-  q.ctas = std::min(q.ctas, chunk_parts(q.chunk * S, q.stage_rows, q.ctas));
-  q.slots = (long long)q.chunks * (2ll * q.ctas + q.chunk);
+  q.ctas = chunk_parts(q.chunk * S, q.stage_rows, stream_ctas() / q.teams);
+  q.slots = (long long)q.chunks * (q.ctas + q.chunk);
   q.ok = slices < (1ll << 30) && units < 2000000000ll && S * q.chunk < (1ll << 40) &&
          q.slots < (1ll << 31);
   q.fan = 1;
@@ -513,7 +504,7 @@ Layout layout(const Plan& q, int B, int C, int G, bool backward) {
   l.set_part = take(sizeof(double2) * (size_t)(backward ? C : G) * B * q.sets);
   if (backward) {
     l.bpart = take(sizeof(float2) * (size_t)C * q.units);
-    l.sums = take(sizeof(double2) * (size_t)C * std::max(B, q.ctas));
+    l.sums = take(sizeof(double2) * (size_t)C * std::max(B, q.ctas * q.teams));
     l.coef = take(sizeof(float4) * (size_t)B * G);
   }
   l.total = at;
@@ -605,13 +596,13 @@ bool feature_norm(const void* x, const void* dy, const void* weight, const void*
   p.sets = q.sets;
   p.units = q.units;
   p.lag = q.lag;
+  p.teams = q.teams;
   p.ctas = q.ctas;
   p.stage_rows = q.stage_rows;
   p.chunk = q.chunk;
   p.chunks = q.chunks;
   p.tickets = out ? 2 * q.units : q.units;
-  const int full = 16 / (int)dtype_bytes(dtype);
-  const bool stream = !q.samples && C <= kStreamChannels && vec_width(dtype, C, x, out, dy) == full;
+  const bool stream = !q.samples && streams(C, G, dtype, vec_width(dtype, C, x, out, dy));
   p.ticket = reinterpret_cast<uint32_t*>(w);
   p.done = p.ticket + 2;
   p.sets_done = p.done + (size_t)B * q.sets;
@@ -631,9 +622,9 @@ bool feature_norm(const void* x, const void* dy, const void* weight, const void*
   if (!stream) return launch(p, dtype, backward, q.samples, s);
   if (!stream_norm(p, dtype, backward, s)) return false;
   if (!backward) return true;
-  if (dtype == LCB200_F32) return launch_params<float>(p, p.ctas, s);
-  if (dtype == LCB200_F16) return launch_params<__half>(p, p.ctas, s);
-  return launch_params<__nv_bfloat16>(p, p.ctas, s);
+  if (dtype == LCB200_F32) return launch_params<float>(p, p.ctas * p.teams, s);
+  if (dtype == LCB200_F16) return launch_params<__half>(p, p.ctas * p.teams, s);
+  return launch_params<__nv_bfloat16>(p, p.ctas * p.teams, s);
 }
 
 int feature_device_status(bool reset) {

@@ -13,16 +13,17 @@
 // needed before the first output, so a sample is read twice; see the launchers
 // for how the second read comes out of L2.
 //
-// Numerics. A thread sums x - K and (x - K)^2 in float32 over its few dozen
-// rows, K being its first value of the channel: what a far-off K costs is
-// bounded by K's own share of the variance. Everything beyond a thread
-// (partial sums, mean, 1/std, the per-channel factors) is float64, so the sums
-// of different slices add without cancellation and the result does not depend
-// on the order the slices finish in: partial sums have slots of their own and
-// are added in a fixed order, with no float atomics.
-// z = x a + b with a = gamma r, b = beta - mu a split into two floats each,
-// which leaves the sign of z exact to ~2^-48: a rectifier's gradient jumps
-// there, and forward and backward must agree on the side.
+// Numerics. sum x and sum x^2 are float64 from the first addition on: every x and x^2
+// is exact there, and mean^2 / var can reach 1e8 before the cancellation in var costs
+// what float32 holds. (Float32 sums of (x - K)^2 over 110 rows left 1/std 1.7e-7 off for
+// bfloat16 maps: squares of odd integers are 1 modulo 8, so their roundings do not
+// average out.) That matters because a rectifier's gradient jumps at z = 0: with 1.7e-7,
+// one training step in three of a 67 million element map had elements on the wrong
+// side. The backward therefore takes z = x a + b with a = gamma r, b = beta - mu a as
+// pairs of floats, whose sign is that of the float64 value but for ~2^-45.
+// The backward's own sums are float32 within a thread and float64 beyond. Partial sums
+// have slots of their own and are added in a fixed order, with no float atomics: results
+// repeat bit for bit.
 #pragma once
 
 #include "feature_common.cuh"
@@ -58,7 +59,8 @@ struct NormArgs {
   uint32_t units, lag;  // B * slices; units between a first pass and its second
   uint32_t tickets;     // 2 * units, or units without a second pass (out null)
   // streamed kernels (see norm_stream.cu)
-  int ctas, stage_rows;
+  int teams, ctas;      // teams of CTAs, CTAs of a team
+  int stage_rows;
   int chunk, chunks;    // samples of a chunk
   // workspace
   uint32_t* ticket;     // [2]: next unit, finished samples
@@ -75,11 +77,10 @@ struct NormArgs {
   DropArgs drop;
 };
 
-// Runs of a chunk of the streamed kernels: two a CTA, one where that would leave less
-// than two stages a run, fewer where it would leave less than a stage.
+// Runs of a chunk of the streamed kernels: one a CTA, fewer where that would leave less
+// than a stage.
 __host__ __device__ inline int chunk_parts(long long rows, int stage_rows, int ctas) {
   const long long stages = (rows + stage_rows - 1) / stage_rows;
-  if (stages >= 4ll * ctas) return 2 * ctas;
   return (int)(stages < ctas ? stages : ctas);
 }
 
@@ -312,7 +313,7 @@ __device__ void param_grads(const NormArgs& p, double2* sm) {
   });
 }
 
-// ---- the kernels: both passes of every chunk --------------------------------------------
+// ---- the plain kernels' order of work --------------------------------------------
 // CTAs draw units from a ticket counter in the order
 //   first(0) ... first(lag - 1) | first(lag), second(0), first(lag + 1), second(1), ... |
 //   second(units - lag) ... second(units - 1)

@@ -2,15 +2,15 @@
 //
 // HBM bound, so the aim is loads that never pause and few instructions a vector
 // (a pass of 16-bit maps has about 90 issue slots per 16 bytes read and written
-// before it falls behind HBM). One CTA per multiprocessor. The rows of a chunk of
-// samples are divided evenly over the CTAs; a CTA makes its first pass (sums) over its
-// rows of a chunk and later its second pass (outputs), by then out of L2. A producer
-// warp copies the rows into a ring of stages with bulk copies, running on across
-// passes; the other warps do the arithmetic, two float32 operations an instruction.
+// before it falls behind HBM). The rows of a chunk of samples are divided evenly over
+// a team of CTAs; a CTA makes its first pass (sums) over its rows of a chunk and then
+// its second pass (outputs), by then out of L2. A producer warp copies the rows into a
+// ring of stages with bulk copies, running on across passes; the other warps do the
+// arithmetic, two float32 operations an instruction.
 //
-// Order of a CTA: first(0) | first(1) a, second(0), first(1) b | first(2) a, second(1),
-// first(2) b | ... | second(last): while a chunk's sums travel between the CTAs,
-// everybody is in half a first pass of the next chunk.
+// Between the passes the team's CTAs wait for each other's sums, 5 to 6 us. So there are
+// two teams, one CTA of each on every multiprocessor, that take the chunks in turn: while
+// one waits, the other streams, and reads of one overlap writes of the other.
 //
 // The sums travel through 16-byte entries that are written whole and start out as all
 // ones: a reader polls the entry itself, so no fence, counter or flag stands between a
@@ -25,10 +25,11 @@
 namespace lcb200 {
 namespace {
 
-constexpr int kS = 512;          // arithmetic threads
+constexpr int kS = 256;          // arithmetic threads
 constexpr int kBlock = kS + 32;  // and the producer warp
-// Vectors of a thread per stage and map: 32 KB stages. A stage costs about 570 cycles
-// from barrier to barrier however small it is: reading 531 MB with one CTA a
+constexpr int kPerSm = 2;        // CTAs of a multiprocessor
+// Vectors of a thread per stage and map: 16 KB stages. A stage costs a CTA about 570
+// cycles from barrier to barrier however small it is: reading 531 MB with one CTA a
 // multiprocessor takes 264 us in 4 KB stages, 141 in 8, 90 in 16 and 86 in 32 KB.
 template <int NM> constexpr int kVecs = 4 / NM;
 
@@ -190,9 +191,9 @@ __device__ void ring_init(RingShared<NM, STAGES>& r) {
 
 // ---- the division of the work -----------------------------------------------------------
 // Chunk k: samples [k m, k m + count), its rows cut into `parts` runs of equal length
-// (to a row), run q starting at row q rows / parts. CTA i has run i, or 2 i and 2 i + 1
-// (its halves a and b). A run is cut again where a sample ends: segments, the s-th
-// sample's in run q with slot q + s of the chunk's.
+// (to a row), run q starting at row q rows / parts and belonging to CTA q of team
+// k % teams. A run is cut again where a sample ends: segments, the s-th sample's in run q
+// with slot q + s of the chunk's.
 struct Chunk {
   int first, count, parts;
   long long rows;
@@ -202,7 +203,7 @@ struct Chunk {
     count = min(p.chunk, p.B - first);
     rows = count * p.S;
     parts = chunk_parts(rows, p.stage_rows, p.ctas);
-    slots = (long long)k * (2 * p.ctas + p.chunk);
+    slots = (long long)k * (p.ctas + p.chunk);
   }
   __device__ __forceinline__ long long start(int q) const {
     return (long long)((unsigned long long)q * (unsigned long long)rows / (unsigned)parts);
@@ -211,20 +212,17 @@ struct Chunk {
   __device__ __forceinline__ int run_of(long long r) const {
     return (int)(((unsigned long long)(r + 1) * (unsigned)parts - 1) / (unsigned long long)rows);
   }
-  __device__ __forceinline__ bool halves(const NormArgs& p) const { return parts > p.ctas; }
 };
 
 // seg(sample of the chunk, first row, end row within the sample) for rows
-// [start, end) of a chunk.
+// [start, end) of a chunk, backwards if `back`.
 template <typename F>
 __device__ __forceinline__ void each_segment(const NormArgs& p, long long start, long long end,
-                                             F seg) {
-  int s = (int)(start / p.S);
-  long long r = start - s * p.S;
-  for (long long left = end - start; left > 0; ++s, r = 0) {
-    const long long stop = min(p.S, r + left);
-    seg(s, r, stop);
-    left -= stop - r;
+                                             bool back, F seg) {
+  const int s0 = (int)(start / p.S), s1 = (int)((end - 1) / p.S);
+  for (int i = 0; i <= s1 - s0; ++i) {
+    const int s = back ? s1 - i : s0 + i;
+    seg(s, max(start - s * p.S, 0ll), min(end - s * p.S, p.S));
   }
 }
 
@@ -239,41 +237,34 @@ __device__ void produce(const NormArgs& p, RingShared<NM, STAGES>& r, const T* m
   auto claim = [&]() {
     return tc::mbar_wait(&r.empty[n % STAGES], ((n / STAGES) & 1) ^ 1, &r.abort);
   };
-  // runs q to q + runs - 1, as one
-  auto run = [&](const Chunk& c, int q, int runs, bool second) {
+  auto run = [&](const Chunk& c, int q, bool second) {
     if (q >= c.parts) return;
     const uint64_t policy = second ? go : stay;
-    each_segment(p, c.start(q), c.start(q + runs), [&](int s, long long row, long long end) {
-      const int seg = (int)(c.slots + q + s), seg_rows = (int)(end - row);
-      const int flags = (second ? kSecond : 0) | (row == 0 ? kTop : 0);
-      long long off = ((long long)(c.first + s) * p.S + row) * p.C;
-      while (row < end && good && (good = claim())) {
+    // a second pass runs backwards: what was read last is what L2 still holds
+    each_segment(p, c.start(q), c.start(q + 1), second, [&](int s, long long r0, long long r1) {
+      const int seg = (int)(c.slots + q + s), seg_rows = (int)(r1 - r0);
+      const int stages = (seg_rows + p.stage_rows - 1) / p.stage_rows;
+      const int flags = (second ? kSecond : 0) | (r0 == 0 ? kTop : 0);
+      for (int t = 0; t < stages && good && (good = claim()); ++t) {
         const int at = n % STAGES;
-        const int rows = (int)min((long long)p.stage_rows, end - row);
+        const long long row = r0 + (long long)(second ? stages - 1 - t : t) * p.stage_rows;
+        const int rows = (int)min((long long)p.stage_rows, r1 - row);
         const uint32_t bytes = (uint32_t)(rows * p.C * sizeof(T));
-        row += rows;
+        const long long off = ((long long)(c.first + s) * p.S + row) * p.C;
         r.info[at] = StageInfo{off, rows, c.first + s, seg, seg_rows,
-                               flags | (row == end ? kLast : 0)};
+                               flags | (t == stages - 1 ? kLast : 0)};
         tc::mbar_arrive_expect_tx(&r.full[at], bytes * NM);
         bulk_copy(r.data[at][0], m0 + off, bytes, &r.full[at], policy);
         if (NM > 1) bulk_copy(r.data[at][NM - 1], m1 + off, bytes, &r.full[at], policy);
-        off += (long long)rows * p.C;
         ++n;
       }
     });
   };
-  const int i = blockIdx.x;
-  for (int k = 0; k <= p.chunks && good; ++k) {
-    const bool some = k < p.chunks;
-    const Chunk c(p, some ? k : 0);
-    const bool two = c.halves(p);
-    if (some) run(c, two ? 2 * i : i, 1, false);
-    if (k > 0 && p.out) {
-      const Chunk before(p, k - 1);
-      if (before.halves(p)) run(before, 2 * i, 2, true);
-      else run(before, i, 1, true);
-    }
-    if (some && two) run(c, 2 * i + 1, 1, false);
+  const int q = blockIdx.x % p.ctas;
+  for (int k = blockIdx.x / p.ctas; k < p.chunks && good; k += p.teams) {
+    const Chunk c(p, k);
+    run(c, q, false);
+    if (p.out) run(c, q, true);
   }
   if (good && claim()) {
     r.info[n % STAGES].flags = kEnd;
@@ -381,42 +372,33 @@ __device__ __forceinline__ void sample_sums(const NormArgs& p, int b, volatile i
 }
 
 // ---- forward -------------------------------------------------------------------------
-// WHOLE: a vector lies in one group, so its V channels share the sums' K.
+// WHOLE: a vector lies in one group, so its V channels share their sums.
 template <typename T, bool WHOLE>
 struct ForwardShared {
-  static constexpr int kV = 16 / sizeof(T), kStages = 4;
+  static constexpr int kV = 16 / sizeof(T), kStages = WHOLE ? 5 : 4;
   RingShared<1, kStages> ring;
-  float sums[3][kS * (WHOLE ? 1 : kV)];  // K, sum (x - K), sum (x - K)^2 of each thread
-  double2 stats[1];                      // [G] of the second pass's sample
+  double2 sums[kS * (WHOLE ? 1 : kV)];  // (sum x, sum x^2) of each thread
+  double2 stats[1];                     // [G] of the second pass's sample
 };
 
 template <typename T, bool WHOLE, typename C>
 __device__ __forceinline__ bool stats_unit(const NormArgs& p, const Place& at, C& in,
                                            ForwardShared<T, WHOLE>& sh) {
-  constexpr int V = 16 / sizeof(T), N = WHOLE ? 1 : V;
-  float2 k[V / 2], s[V / 2], q[V / 2];  // k: minus K
+  constexpr int V = 16 / sizeof(T), N = WHOLE ? 1 : V, A = WHOLE ? 2 : V;
+  double s[A], q[A];
 #pragma unroll
-  for (int v = 0; v < V / 2; ++v) s[v] = q[v] = k[v] = twice(0.f);
-  const int seg = in.now.seg, rows = in.now.seg_rows;
-  bool first = true;
+  for (int v = 0; v < A; ++v) s[v] = q[v] = 0.0;
+  const int seg = in.now.seg;
   for (;;) {
     const uint4* data = in.map(0);
-    if (first && at.on && at.row < in.now.rows) {
-      float2 f[V / 2];
-      Vec2<T>::unpack(data[threadIdx.x], f);
-#pragma unroll
-      for (int v = 0; v < V / 2; ++v)
-        k[v] = WHOLE ? twice(-f[0].x) : make_float2(-f[v].x, -f[v].y);
-    }
-    first = false;
     stage_rows<kVecs<1>>(at, in.now.rows, [&](int i, int) {
       float2 f[V / 2];
       Vec2<T>::unpack(data[i], f);
 #pragma unroll
-      for (int v = 0; v < V / 2; ++v) {
-        const float2 d = add2(f[v], k[v]);
-        s[v] = add2(s[v], d);
-        q[v] = fma2(d, d, q[v]);
+      for (int v = 0; v < V; ++v) {
+        const double x = v & 1 ? f[v / 2].y : f[v / 2].x;
+        s[v % A] += x;
+        q[v % A] = fma(x, x, q[v % A]);
       }
     });
     const bool last = in.now.flags & kLast;
@@ -425,28 +407,14 @@ __device__ __forceinline__ bool stats_unit(const NormArgs& p, const Place& at, C
     if (!in.open()) return false;
   }
   if (WHOLE) {
-    float2 ss = s[0], qq = q[0];
-#pragma unroll
-    for (int v = 1; v < V / 2; ++v) {
-      ss = add2(ss, s[v]);
-      qq = add2(qq, q[v]);
-    }
-    sh.sums[0][threadIdx.x] = -k[0].x;
-    sh.sums[1][threadIdx.x] = ss.x + ss.y;
-    sh.sums[2][threadIdx.x] = qq.x + qq.y;
+    sh.sums[threadIdx.x] = make_double2(s[0] + s[1], q[0] + q[1]);
   } else {
 #pragma unroll
-    for (int v = 0; v < V / 2; ++v) {
-      const int at2 = threadIdx.x * V / 2 + v;
-      reinterpret_cast<float2*>(sh.sums[0])[at2] = make_float2(-k[v].x, -k[v].y);
-      reinterpret_cast<float2*>(sh.sums[1])[at2] = s[v];
-      reinterpret_cast<float2*>(sh.sums[2])[at2] = q[v];
-    }
+    for (int v = 0; v < N; ++v) sh.sums[threadIdx.x * N + v] = make_double2(s[v], q[v]);
   }
   stream_sync();
-  // One group by `width` lanes: sum x = s + n K, sum x^2 = q + 2 K s + n K^2 in
-  // float64, n values an entry.
-  const int ne = at.nc * N, gw = p.Cg * N / V, full = rows / at.rp, rest = rows % at.rp;
+  // one group by `width` lanes
+  const int ne = at.nc * N, gw = p.Cg * N / V;
   const int width = min(32, max(1, pow2_below(min(at.rp * gw, kS / min(p.G, kS)))));
   const int lane = threadIdx.x % width;
   for (int g0 = 0; g0 < p.G; g0 += kS / width) {
@@ -454,14 +422,10 @@ __device__ __forceinline__ bool stats_unit(const NormArgs& p, const Place& at, C
     double2 t = make_double2(0.0, 0.0);
     if (g < p.G) {
       for (int i = lane; i < at.rp * gw; i += width) {
-        const int r = i / gw, e = r * ne + g * gw + (i - r * gw);
-        const int steps = full + (r < rest);
-        if (steps > 0) {
-          const double n = steps * (V / N);
-          const double k = sh.sums[0][e], s = sh.sums[1][e], q = sh.sums[2][e];
-          t.x += s + n * k;
-          t.y += q + k * (2.0 * s + n * k);
-        }
+        const int r = i / gw;
+        const double2 e = sh.sums[r * ne + g * gw + (i - r * gw)];
+        t.x += e.x;
+        t.y += e.y;
       }
     }
     t = lanes_sum(t, width);
@@ -556,7 +520,7 @@ __device__ __forceinline__ bool apply_unit(const NormArgs& p, const Place& at, C
 }
 
 template <typename T, bool WHOLE, bool DROP>
-__global__ void __launch_bounds__(kBlock, 1) norm_forward_stream(NormArgs p) {
+__global__ void __launch_bounds__(kBlock, kPerSm) norm_forward_stream(NormArgs p) {
   extern __shared__ __align__(128) unsigned char smem[];
   auto& sh = *reinterpret_cast<ForwardShared<T, WHOLE>*>(smem);
   drop_keep_stream(p.drop);
@@ -582,7 +546,7 @@ __global__ void __launch_bounds__(kBlock, 1) norm_forward_stream(NormArgs p) {
 // RECT: a rectifier, whose side needs z to more than float32 (see norm_common.cuh).
 template <typename T, bool WHOLE>
 struct BackwardShared {
-  static constexpr int kV = 16 / sizeof(T), kStages = 4;
+  static constexpr int kV = 16 / sizeof(T), kStages = 5;
   RingShared<2, kStages> ring;
   float2 sums[kS * kV];  // sum dz, sum dz (x - mu)
   float4 coef[1];        // [G] of the second pass's sample
@@ -792,7 +756,7 @@ __device__ __forceinline__ bool grad_input_unit(const NormArgs& p, const Place& 
 }
 
 template <typename T, bool WHOLE, bool RECT, bool DROP>
-__global__ void __launch_bounds__(kBlock, 1) norm_backward_stream(NormArgs p) {
+__global__ void __launch_bounds__(kBlock, kPerSm) norm_backward_stream(NormArgs p) {
   extern __shared__ __align__(128) unsigned char smem[];
   auto& sh = *reinterpret_cast<BackwardShared<T, WHOLE>*>(smem);
   ring_init(sh.ring);
@@ -804,13 +768,16 @@ __global__ void __launch_bounds__(kBlock, 1) norm_backward_stream(NormArgs p) {
   }
   const Place at(p.C / (16 / (int)sizeof(T)), 0, kS);
   Consumer<2, BackwardShared<T, WHOLE>::kStages> in(sh.ring);
-  bool started = false;
+  bool started = false;  // whether this CTA's row of parameter sums holds something
   while (in.open()) {
     if (in.now.flags & kSecond
             ? !grad_input_unit<T, WHOLE, RECT, DROP>(p, at, in, sh.coef)
             : !grad_sums_unit<T, WHOLE, RECT, DROP>(p, at, in, sh.sums, &started))
       break;
   }
+  if (!started && (p.dweight || p.dbias))
+    for (int c = threadIdx.x; c < p.C; c += kS)
+      p.sums[(long long)blockIdx.x * p.C + c] = make_double2(0.0, 0.0);
   if (!(in.now.flags & kEnd)) sh.ring.abort = 1;
 }
 
@@ -821,7 +788,7 @@ bool launch_kernel(K kernel, size_t smem, const NormArgs& p, const char* what, c
   if (!ensure_smem_attr((const void*)kernel, smem + 1024)) return false;
   NormArgs args = p;
   void* argv[] = {&args};
-  if (cudaLaunchCooperativeKernel((const void*)kernel, dim3(p.ctas), dim3(kBlock), argv, smem,
+  if (cudaLaunchCooperativeKernel((const void*)kernel, dim3(p.ctas * p.teams), dim3(kBlock), argv, smem,
                                   s) != cudaSuccess)
     return check_launch(what);
   count_launch();
@@ -857,6 +824,8 @@ bool stream_norm(const NormArgs& p, int dtype, bool backward, cudaStream_t s) {
   if (dtype == LCB200_F16) return launch_t<__half>(p, backward, s);
   return launch_t<__nv_bfloat16>(p, backward, s);
 }
+
+int stream_ctas() { return device_sms() * kPerSm; }
 
 int stream_stage_rows(int C, int dtype, bool backward) {
   const int cols = std::max(1, C / (16 / (int)dtype_bytes(dtype)));

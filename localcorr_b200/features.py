@@ -235,25 +235,25 @@ def group_norm_backward(grad_y, x, weight, bias, stats, used, num_groups, activa
 # ---------------------------------------------------------------------------
 
 class GroupNormFunction(torch.autograd.Function):
-    """group_norm with its gradients; saves x and the float64 statistics."""
+    """group_norm with its gradients; saves x and the float64 statistics. ``params``: the
+    arguments of :func:`group_norm_forward` between bias and rng."""
 
     @staticmethod
-    def forward(ctx, x, weight, bias, num_groups, eps, activation, negative_slope, p, channel,
-                rng, seed, offset):
+    def forward(ctx, x, weight, bias, params, rng, seed, offset):
         x = x.contiguous()
-        y, stats, used = group_norm_forward(x, weight, bias, num_groups, eps, activation,
-                                            negative_slope, p, channel, rng, seed, offset)
-        ctx.save_for_backward(x, weight, bias, stats, used)
-        ctx.params = (num_groups, activation, negative_slope, p, channel)
+        y, ctx.stats, ctx.used = group_norm_forward(x, weight, bias, *params, rng, seed, offset)
+        ctx.save_for_backward(x, weight, bias)
+        ctx.params = params
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_y):
-        need = ctx.needs_input_grad
-        grads = group_norm_backward(grad_y, *ctx.saved_tensors, *ctx.params, need[0], need[1],
-                                    need[2])
-        return (*grads, None, None, None, None, None, None, None, None, None)
+        num_groups, _, activation, negative_slope, p, channel = ctx.params
+        nx, nw, nb = ctx.needs_input_grad[:3]
+        return (*group_norm_backward(grad_y, *ctx.saved_tensors, ctx.stats, ctx.used, num_groups,
+                                     activation, negative_slope, p, channel, nx, nw, nb),
+                None, None, None, None)
 
 
 class DropoutFunction(torch.autograd.Function):
@@ -261,15 +261,14 @@ class DropoutFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, residual, p, channel, rng, seed, offset):
-        y, used = dropout_forward(x, residual, p, channel, rng, seed, offset)
-        ctx.save_for_backward(used)
+        y, ctx.used = dropout_forward(x, residual, p, channel, rng, seed, offset)
         ctx.params = (p, channel)
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_y):
-        gx = (dropout_backward(grad_y, *ctx.saved_tensors, *ctx.params)
+        gx = (dropout_backward(grad_y, ctx.used, *ctx.params)
               if ctx.needs_input_grad[0] else None)
         gr = grad_y if ctx.needs_input_grad[1] else None
         return gx, gr, None, None, None, None, None
@@ -298,15 +297,15 @@ def group_norm(x, num_groups, weight=None, bias=None, eps=1e-5, activation="none
     _check_norm(x, num_groups, weight, bias, eps, activation, negative_slope)
     p = _check_dropout(p, rng, dropout_mode, x, "group_norm")
     tensor, seed, offset = _split_rng(rng)
-    args = (x, weight, bias, num_groups, float(eps), activation, float(negative_slope), p,
-            dropout_mode == "channel", tensor, seed, offset)
+    params = (num_groups, float(eps), activation, float(negative_slope), p,
+              dropout_mode == "channel")
     if torch.compiler.is_compiling():
-        return torch.ops.localcorr.group_norm(*args)[0]
+        return torch.ops.localcorr.group_norm(x, weight, bias, *params, tensor, seed, offset)[0]
     if torch.is_grad_enabled() and (x.requires_grad
                                     or (weight is not None and weight.requires_grad)
                                     or (bias is not None and bias.requires_grad)):
-        return GroupNormFunction.apply(*args)
-    return group_norm_forward(*args)[0]
+        return GroupNormFunction.apply(x, weight, bias, params, tensor, seed, offset)
+    return group_norm_forward(x, weight, bias, *params, tensor, seed, offset)[0]
 
 
 def dropout(x, p, rng, residual=None, mode="element"):

@@ -1,13 +1,13 @@
 """group_norm and dropout on the GPU against the 64-bit oracle.
 
-Tolerances. u = eps(dtype) / 2 is the final rounding. Inside, a thread sums at
-most 64 rows of x - K in float32, so a mean is off by at most 64 u32 mean|x - K|
-with u32 = 2^-24, which is below 2^-16 standard deviations (mean|x - K| <= 4
-std for these inputs), and 1/std by as much relatively. Hence z is off by
-2^-16 |gamma| (|xhat| + 1) and 2^-22 |z| (two products, a sum, exp and a quotient
-of 2 ulp each), the activations have slope at most 1.1, and each term of a
-gradient carries the same relative error (2^-15 covers statistics and sums).
-A rectifier's gradient may take either side where |z| is below z's tolerance.
+Tolerances. u = eps(dtype) / 2 is the final rounding. The statistics are float64 sums,
+off by 2^-45 at most here. z = (x - mu) a + c takes a handful of float32 roundings, below
+2^-21 |gamma| (|xhat| + 1) + 2^-22 |z| with the exp and quotient of 2 ulp each. The
+backward's sums are float32 over at most 256 rows of a thread and float64 beyond, so
+they carry 2^-16 of the sum of their terms' magnitudes. z's tolerance is taken as
+2^-16 |gamma| (|xhat| + 1) + 2^-22 |z| throughout, which covers both; the activations
+have slope at most 1.1. A rectifier's gradient may take either side where |z| is below
+z's tolerance here; that it takes float64's is test_rectifiers_take_the_float64_side.
 """
 
 import math
@@ -128,6 +128,13 @@ def _check_norm(x, w, b, dy, groups, act, p=0.0, stream=(7, 3), mode="element", 
     ((5, 3, 3, 12), 12),       # instance norm
     ((1, 17, 4104), 8),        # wider than a CTA, groups cut by its column blocks
     ((2, 2, 2100), 1),         # one group across column blocks
+    ((2, 3000, 33), 11),       # divided, element by element
+    ((1, 90, 4104), 8),        # divided, wider than a CTA
+    ((3, 41, 53, 64), 8),      # divided, streamed
+    ((2, 37, 2048), 16),       # streamed in 16 bits, too wide in 32
+    ((3, 65, 1032), 3),        # rows no thread tiling fits evenly
+    ((2, 150, 512), 512),      # the most groups that are streamed
+    ((2, 150, 520), 520),      # one vector more
 ])
 def test_norm_against_oracle(dtype, act, shape, groups):
     x, w, b, dy = _norm_case(shape, DTYPES[dtype])
@@ -150,7 +157,8 @@ def test_norm_groups_and_batches(groups, batch):
 @pytest.mark.parametrize("mode", ["element", "channel"])
 @pytest.mark.parametrize("dtype", list(DTYPES))
 @pytest.mark.parametrize("shape,groups", [((2, 19, 23, 64), 8), ((3, 7, 33), 3), ((2, 5, 12), 2),
-                                          ((2, 5, 6), 1)])
+                                          ((2, 5, 6), 1), ((3, 41, 53, 64), 8),
+                                          ((2, 1500, 100), 20), ((2, 2500, 33), 3)])
 def test_norm_with_dropout(mode, dtype, shape, groups):
     x, w, b, dy = _norm_case(shape, DTYPES[dtype], seed=4)
     _check_norm(x, w, b, dy, groups, "relu", p=0.3, stream=(2 ** 62 + 12345, 2 ** 40 + 9),
@@ -170,8 +178,7 @@ def test_norm_parameters_of_the_maps_type(dtype):
 
 
 def test_norm_offset_far_above_spread():
-    # mean 1000, spread ~1: float32 inputs hold it to 2^-15 of the spread by themselves; what
-    # the sums lose is relative to x - K, not to x
+    # mean 1000, spread ~1: the difference to the mean is taken before anything is scaled
     x, w, b, dy = _norm_case((2, 40, 40, 32), torch.float32, shift=1000.0)
     _check_norm(x, w, b, dy, 4, "silu")
 
@@ -180,7 +187,7 @@ def test_norm_constant_group_and_eps():
     x = torch.full((2, 30, 16), 3.25, dtype=torch.float16, device=DEV)
     b = torch.linspace(-1, 1, 16, device=DEV)
     y = lc.group_norm(x, 4, None, b)
-    # xhat = 0 exactly: x - K = 0, and mean * a cancels to below 2^-40
+    # the variance cancels to below 2^-40 of x^2, and x - mean is 0
     torch.testing.assert_close(y.float(), b.half().float().expand(2, 30, 16), rtol=0,
                                atol=2.0 ** -11)
     y = lc.group_norm(x[:, :1, :4].contiguous(), 4, None, b[:4])  # groups of one value
@@ -188,9 +195,10 @@ def test_norm_constant_group_and_eps():
                                atol=2.0 ** -11)
 
 
+@pytest.mark.parametrize("rows", [21, 2100])
 @pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
-def test_norm_keeps_what_is_not_finite_in_its_group(bad):
-    x, w, b, dy = _norm_case((2, 21, 24), torch.float32)
+def test_norm_keeps_what_is_not_finite_in_its_group(bad, rows):
+    x, w, b, dy = _norm_case((2, rows, 24), torch.float32)
     clean = lc.group_norm(x.to(DEV), 3, w.to(DEV), b.to(DEV), activation="relu").cpu()
     x[1, 7, 9] = bad
     xg = x.to(DEV).requires_grad_(True)
@@ -202,6 +210,35 @@ def test_norm_keeps_what_is_not_finite_in_its_group(bad):
     (g,) = torch.autograd.grad(lc.group_norm(xg, 3), xg, dy.to(DEV))
     assert bool(g[0].isfinite().all() and g[1, :, :8].isfinite().all()
                 and g[1, :, 16:].isfinite().all())
+
+
+@pytest.mark.parametrize("shape,groups", [((4, 9000, 64), 64), ((3, 20000, 128), 16),
+                                          ((2, 5000, 35), 5), ((6, 60, 96), 12)])
+@pytest.mark.parametrize("dtype", list(DTYPES))
+def test_rectifiers_take_the_float64_side(dtype, shape, groups):
+    # with an output gradient of ones the bias's gradient counts the elements above the
+    # corner: whole numbers, to be met exactly. float64 itself decides where |z| > 2^-40.
+    x, w, b, dy = _norm_case(shape, DTYPES[dtype], seed=31)
+    xhat, _ = oracle.normalised(x.double(), groups, 1e-5)
+    z = xhat * w.double() + b.double()
+    assert float(z.abs().min()) > 2.0 ** -40
+    gb = b.to(DEV).requires_grad_(True)
+    y = lc.group_norm(x.to(DEV), groups, w.to(DEV), gb, activation="relu")
+    (count,) = torch.autograd.grad(y, gb, torch.ones_like(y))
+    assert torch.equal(count.double().cpu(), (z > 0).sum((0, 1)).double())
+
+
+@pytest.mark.parametrize("rows", [100, 4000])
+def test_norm_statistics_are_float64(rows):
+    x, w, b, dy = _norm_case((3, rows, 64), torch.bfloat16, seed=32, shift=50.0)
+    _, stats, _ = features.group_norm_forward(x.to(DEV), None, None, 64, 1e-5, "none", 0.0, 0.0,
+                                              False, None, 0, 0)
+    v = x.double()
+    mean, var = v.mean(1), v.var(1, correction=0)
+    # n 2^-53 of the sums; mean^2 / var is below 2^13, which the cancellation costs
+    torch.testing.assert_close(stats[..., 0].cpu(), mean, rtol=2.0 ** -40, atol=0)
+    torch.testing.assert_close(stats[..., 1].cpu(), 1 / torch.sqrt(var + 1e-5), rtol=2.0 ** -26,
+                               atol=0)
 
 
 def test_norm_large_float16_values():
@@ -236,8 +273,9 @@ def test_norm_gradient_against_differences():
         assert abs(diff[0] - want) <= tol, (i, diff, want, tol)
 
 
-def test_norm_strides_alignment_and_expanded_gradients():
-    x, w, b, dy = _norm_case((2, 10, 12, 40), torch.float16)
+@pytest.mark.parametrize("size", [(10, 12), (50, 60)])
+def test_norm_strides_alignment_and_expanded_gradients(size):
+    x, w, b, dy = _norm_case((2, *size, 40), torch.float16)
     want = lc.group_norm(x.to(DEV), 5, w.to(DEV), b.to(DEV), activation="relu")
     nchw = x.to(DEV).permute(0, 3, 1, 2).contiguous()                  # NCHW: copied
     assert torch.equal(lc.group_norm(nchw.permute(0, 2, 3, 1), 5, w.to(DEV), b.to(DEV),
@@ -258,8 +296,9 @@ def test_norm_strides_alignment_and_expanded_gradients():
     assert torch.equal(g0, g1)
 
 
-def test_norm_one_needed_gradient():
-    x, w, b, dy = (t.to(DEV) for t in _norm_case((2, 10, 40), torch.float16))
+@pytest.mark.parametrize("shape", [(2, 10, 40), (3, 2000, 40), (2, 3000, 35)])
+def test_norm_one_needed_gradient(shape):
+    x, w, b, dy = (t.to(DEV) for t in _norm_case(shape, torch.float16))
     full = [t.clone().requires_grad_(True) for t in (x, w, b)]
     want = torch.autograd.grad(lc.group_norm(full[0], 5, full[1], full[2], activation="silu"),
                                full, dy)
@@ -271,12 +310,14 @@ def test_norm_one_needed_gradient():
         assert torch.equal(got, want[i])
 
 
-def test_norm_repeats_bit_for_bit():
-    x, w, b, dy = (t.to(DEV) for t in _norm_case((4, 60, 70, 64), torch.float16))
+@pytest.mark.parametrize("c", [64, 72, 56, 60])
+def test_norm_repeats_bit_for_bit(c):
+    x, w, b, dy = (t.to(DEV) for t in _norm_case((4, 60, 70, c), torch.float16))
     out = []
     for _ in range(3):
         leaves = [t.clone().requires_grad_(True) for t in (x, w, b)]
-        y = lc.group_norm(leaves[0], 8, leaves[1], leaves[2], activation="relu", p=0.2, rng=(1, 5))
+        y = lc.group_norm(leaves[0], 4, leaves[1], leaves[2], activation="relu", p=0.2,
+                          rng=(1, 5))
         out.append((y.detach(), *torch.autograd.grad(y, leaves, dy)))
     for other in out[1:]:
         assert all(torch.equal(a, o) for a, o in zip(out[0], other))
@@ -388,7 +429,7 @@ def test_norm_beyond_32_bit_offsets():
     assert x.numel() > 1 << 31
     y = lc.group_norm(x, 13, activation="silu")[b - 1]
     alone = lc.group_norm(x[b - 1:].contiguous(), 13, activation="silu")[0]
-    # slices differ: the statistics to 2^-16, then the rounding of either
+    # other runs: the same statistics but for 2^-45, then the rounding of either
     torch.testing.assert_close(y, alone, rtol=2.0 ** -10, atol=2.0 ** -13)
 
 
@@ -421,14 +462,37 @@ def test_every_element_and_offset_draws_its_own():
             assert abs(agree - 0.5) < 5 * 0.5 / math.sqrt(64000)
 
 
+def test_large_maps_of_many_chunks():
+    # several chunks a team, runs that end inside samples: the same sample alone agrees
+    x = torch.empty(13, 61, 1031, 256, dtype=torch.bfloat16, device=DEV).normal_()  # 419 MB
+    w, b = (torch.linspace(0.5, 1.5, 256, device=DEV).requires_grad_(True) for _ in range(2))
+    dy = torch.empty_like(x).normal_()
+    xg = x.requires_grad_(True)
+    y = lc.group_norm(xg, 16, w, b, activation="silu")
+    gx, gw, gb = torch.autograd.grad(y, (xg, w, b), dy)
+    sw = sb = 0
+    for i in range(13):
+        one = x[i:i + 1].detach().requires_grad_(True)
+        yi = lc.group_norm(one, 16, w, b, activation="silu")
+        gi, gwi, gbi = torch.autograd.grad(yi, (one, w, b), dy[i:i + 1])
+        # other runs: the backward's sums to 2^-16, then the rounding of either to 2^-8
+        torch.testing.assert_close(y[i:i + 1], yi, rtol=2.0 ** -7, atol=2.0 ** -12)
+        torch.testing.assert_close(gx[i:i + 1], gi, rtol=2.0 ** -7, atol=2.0 ** -12)
+        sw, sb = sw + gwi.double(), sb + gbi.double()
+    # sums of 817,583 terms of about 1 in float32 pieces of at most a few hundred
+    torch.testing.assert_close(gw.double(), sw, rtol=2.0 ** -16, atol=0.5)
+    torch.testing.assert_close(gb.double(), sb, rtol=2.0 ** -16, atol=0.5)
+
+
 def _train_step(x, w, b, dy, rng):
     y = lc.group_norm(x, 8, w, b, activation="relu", p=0.25, rng=rng)
     y2 = lc.dropout(y, 0.5, rng, residual=y, mode="channel")
     return (y2, *torch.autograd.grad(y2, (x, w, b), dy))
 
 
-def test_captured_training_steps_replay_with_new_draws():
-    x, w, b, dy = (t.to(DEV) for t in _norm_case((3, 33, 21, 64), torch.float16))
+@pytest.mark.parametrize("shape", [(3, 7, 9, 64), (3, 66, 42, 64), (2, 50, 60, 40)])
+def test_captured_training_steps_replay_with_new_draws(shape):
+    x, w, b, dy = (t.to(DEV) for t in _norm_case(shape, torch.float16))
     x, w, b = (t.requires_grad_(True) for t in (x, w, b))
     rng = torch.tensor([31, 0], device=DEV)
     side = torch.cuda.Stream()
