@@ -329,7 +329,8 @@ LCB200_API bool launchLocalCorrB200Dropout(const void* x, const void* residual, 
  * variance over rows and the group's channels), the activation (negative_slope
  * is LEAKY_RELU's), and with p > 0 dropout. weight and bias: [C], either may
  * be NULL (1 and 0), of float32 (param_f32) or of dtype. stats receives
- * [B, groups] pairs of float64 (mean, 1/sqrt(var + eps)), 16-byte aligned. */
+ * [B, groups] pairs of float64 (mean, 1/sqrt(var + eps)), 16-byte aligned. x and y
+ * do not overlap; the workspace is 16-byte aligned, one for each call in flight. */
 LCB200_API size_t localCorrB200GroupNormWorkspaceBytes(int B, long long rows, int C, int groups,
                                                        int dtype, bool backward);
 LCB200_API bool launchLocalCorrB200GroupNormForward(

@@ -16,11 +16,10 @@ namespace {
 
 // ---- forward, first pass: slice sums, and the sample's statistics -----------------
 template <typename T, int V>
-__device__ void stats_slice(const NormArgs& p, int b, int j, double2* sm) {
+__device__ void stats_slice(const NormArgs& p, int b, int j, double2* out, double2* sm) {
   const int cols = p.C / V;
   const long long r0 = j * p.slice_rows, r1 = min(p.S, r0 + p.slice_rows);
   const T* xb = reinterpret_cast<const T*>(p.x) + (long long)b * p.S * p.C;
-  double2* out = p.part + ((long long)b * p.slices + j) * p.G;
   const bool whole = p.Cg % V == 0;  // a vector lies in one group
   const int per = whole ? 1 : V;     // shared entries of a thread
   const int gw = p.Cg * per / V;     // entries of one group and row (whole: Cg / V)
@@ -162,11 +161,10 @@ __device__ __forceinline__ void to_dz(const NormArgs& p, const Affine (&f)[V],
 }
 
 template <typename T, int V, bool DROP>
-__device__ void grad_sums_slice(const NormArgs& p, int b, int j, float2* sm) {
+__device__ void grad_sums_slice(const NormArgs& p, int b, int j, float2* out, float2* sm) {
   const int cols = p.C / V;
   const long long r0 = j * p.slice_rows, r1 = min(p.S, r0 + p.slice_rows);
   const long long base = (long long)b * p.S * p.C;
-  float2* out = p.bpart + ((long long)b * p.slices + j) * p.C;
   DropStream ds;
   if (DROP) ds = drop_stream(p.drop);
   for (int cb = 0; cb < cols; cb += kT) {
@@ -235,7 +233,7 @@ __device__ void grad_sums_slice(const NormArgs& p, int b, int j, float2* sm) {
 
 // ---- backward, second pass --------------------------------------------------------------
 template <typename T, int V, bool DROP>
-__device__ void grad_input_slice(const NormArgs& p, int b, int j) {
+__device__ void grad_input_slice(const NormArgs& p, int b, int j, const float4* coef) {
   const int cols = p.C / V;
   const long long r0 = j * p.slice_rows, r1 = min(p.S, r0 + p.slice_rows);
   const long long base = (long long)b * p.S * p.C;
@@ -249,9 +247,9 @@ __device__ void grad_input_slice(const NormArgs& p, int b, int j) {
     const int c0 = at.col * V;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      const long long g = (long long)b * p.G + (c0 + v) / p.Cg;
-      f[v] = affine<T>(p, __ldg(p.stats + g), c0 + v);
-      const float4 k = __ldcg(p.coef + g);
+      const int g = (c0 + v) / p.Cg;
+      f[v] = affine<T>(p, __ldg(p.stats + (long long)b * p.G + g), c0 + v);
+      const float4 k = __ldcg(coef + g);
       mu[v] = k.x;
       k2[v] = k.y;
       k3[v] = k.z;
@@ -316,7 +314,7 @@ __global__ void __launch_bounds__(kT, kOcc) norm_forward_kernel(NormArgs p) {
   drop_keep_stream(p.drop);
   run_units(p, [&](bool second, int b, int j) {
     if (!second) {
-      stats_slice<T, V>(p, b, j, sm);
+      stats_slice<T, V>(p, b, j, p.part + ((long long)b * p.slices + j) * p.G, sm);
       if (finish_slice(p, b, j, p.part, p.G, sm, [&](int g, double2 t) {
             p.stats[(long long)b * p.G + g] = finish_stats(p, t);
           }))
@@ -335,17 +333,18 @@ __global__ void __launch_bounds__(kT, kOcc) norm_backward_kernel(NormArgs p) {
   double2* smd = reinterpret_cast<double2*>(sm);
   run_units(p, [&](bool second, int b, int j) {
     if (!second) {
-      grad_sums_slice<T, V, DROP>(p, b, j, sm);
+      grad_sums_slice<T, V, DROP>(p, b, j, p.bpart + ((long long)b * p.slices + j) * p.C, sm);
+      double2* sums = p.sums + (long long)b * p.C;
       if (finish_slice(p, b, j, p.bpart, p.C, smd,
-                       [&](int c, double2 t) { finish_channel(p, b, c, t); })) {
-        finish_coef<T>(p, b);
+                       [&](int c, double2 t) { sums[c] = finish_channel(p, b, c, t); })) {
+        finish_coef<T>(p, b, sums, p.coef + (long long)b * p.G);
         publish(p.ready + b);
         if (last_of(p.ticket + 1, p.B)) param_grads<T>(p, smd);
       }
       return true;
     }
     if (!wait_for(p.ready + b)) return false;
-    grad_input_slice<T, V, DROP>(p, b, j);
+    grad_input_slice<T, V, DROP>(p, b, j, p.coef + (long long)b * p.G);
     return true;
   });
 }
@@ -353,16 +352,16 @@ __global__ void __launch_bounds__(kT, kOcc) norm_backward_kernel(NormArgs p) {
 // ---- whole samples ------------------------------------------------------------------------
 // A CTA makes both passes of a sample: nothing to exchange, one ordinary launch, the
 // second read out of L1 and L2. For samples too small to divide and for many small ones.
+// Partial sums, coefficients and sums of the parameters' gradients are the CTA's own.
 template <typename T, int V, bool DROP>
 __global__ void __launch_bounds__(kT, kOcc) norm_forward_samples(NormArgs p) {
   __shared__ double2 sm[kT * V];
   drop_keep_stream(p.drop);
+  double2* part = p.part + (long long)blockIdx.x * p.G;
   for (int b = blockIdx.x; b < p.B; b += gridDim.x) {
-    stats_slice<T, V>(p, b, 0, sm);
-    for (int g = threadIdx.x; g < p.G; g += kT) {
-      const long long i = (long long)b * p.G + g;
-      p.stats[i] = finish_stats(p, __ldcg(p.part + i));
-    }
+    stats_slice<T, V>(p, b, 0, part, sm);
+    for (int g = threadIdx.x; g < p.G; g += kT)
+      p.stats[(long long)b * p.G + g] = finish_stats(p, __ldcg(part + g));
     cta_sync();
     apply_slice<T, V, DROP>(p, b, 0);
   }
@@ -370,20 +369,33 @@ __global__ void __launch_bounds__(kT, kOcc) norm_forward_samples(NormArgs p) {
 
 template <typename T, int V, bool DROP>
 __global__ void __launch_bounds__(kT, kOcc) norm_backward_samples(NormArgs p) {
-  __shared__ __align__(16) float2 sm[kT * (V < 2 ? 2 : V)];  // also kT double2 sums
-  double2* smd = reinterpret_cast<double2*>(sm);
+  __shared__ __align__(16) float2 sm[kT * (V < 2 ? 2 : V)];
+  const long long own = blockIdx.x;
+  float2* bpart = p.bpart + own * p.C;
+  double2 *sums = p.set_part + own * p.C, *total = p.sums + own * p.C;
+  float4* coef = p.coef + own * p.G;
   for (int b = blockIdx.x; b < p.B; b += gridDim.x) {
-    grad_sums_slice<T, V, DROP>(p, b, 0, sm);
-    for (int c = threadIdx.x; c < p.C; c += kT)
-      finish_channel(p, b, c, as_double2(__ldcg(p.bpart + (long long)b * p.C + c)));
-    finish_coef<T>(p, b);
+    grad_sums_slice<T, V, DROP>(p, b, 0, bpart, sm);
+    for (int c = threadIdx.x; c < p.C; c += kT) {
+      const double2 v = finish_channel(p, b, c, as_double2(__ldcg(bpart + c)));
+      sums[c] = v;
+      double2 t = b < (int)gridDim.x ? make_double2(0.0, 0.0) : total[c];
+      t.x += v.x;
+      t.y += v.y;
+      total[c] = t;
+      if (gridDim.x == 1 && b + 1 == p.B) {
+        put_param<T>(p.dbias, p.param_f32, c, t.x);
+        put_param<T>(p.dweight, p.param_f32, c, t.y);
+      }
+    }
+    finish_coef<T>(p, b, sums, coef);
     cta_sync();
-    if (p.out) grad_input_slice<T, V, DROP>(p, b, 0);
+    if (p.out) grad_input_slice<T, V, DROP>(p, b, 0, coef);
+    cta_sync();
   }
-  if (p.B == 1) param_grads<T>(p, smd);
 }
 
-// Weight and bias gradients from per-sample or per-CTA channel sums [n, C]: two channels
+// Weight and bias gradients from the CTAs' channel sums [n, C]: two channels
 // a CTA (a 32-byte sector a row), rows over its threads, a fixed order throughout.
 constexpr int kParamChannels = 2;
 template <typename T>
@@ -479,6 +491,11 @@ Plan make_plan(int B, long long S, int C, int dtype, bool backward) {
   q.slots = (long long)q.chunks * (q.ctas + q.chunk);
   q.ok = slices < (1ll << 30) && units < 2000000000ll && S * q.chunk < (1ll << 40) &&
          q.slots < (1ll << 31);
+  if (q.samples) {
+    q.ctas = (int)std::min<long long>(B, device_sms() * kOcc);
+    q.teams = 1;
+    q.slots = 0;
+  }
   q.fan = 1;
   while ((long long)q.fan * q.fan < slices) ++q.fan;
   q.sets = (int)((slices + q.fan - 1) / q.fan);
@@ -486,10 +503,10 @@ Plan make_plan(int B, long long S, int C, int dtype, bool backward) {
 }
 
 struct Layout {  // byte offsets
-  size_t flags, part, plain, set_part, bpart, sums, coef, total;
+  size_t flags, part, set_part, bpart, sums, coef, total;
 };
-// [0, flags): counters of the plain kernels, from 0. [part, plain): entries of the
-// streamed kernels, from all ones.
+// [0, flags): counters of the plain kernels, set to 0. part: set to all ones for the
+// streamed kernels.
 Layout layout(const Plan& q, int B, int C, int G, bool backward) {
   size_t at = 0;
   auto take = [&](size_t bytes) {
@@ -499,13 +516,15 @@ Layout layout(const Plan& q, int B, int C, int G, bool backward) {
   };
   Layout l{};
   take(l.flags = sizeof(uint32_t) * (2 + (2 + (size_t)q.sets) * B));
-  l.part = take(sizeof(double2) * (size_t)G * std::max<size_t>(q.units, q.samples ? 0 : q.slots));
-  l.plain = at;
-  l.set_part = take(sizeof(double2) * (size_t)(backward ? C : G) * B * q.sets);
+  // whole samples: a row of each for every CTA
+  const size_t rows = q.samples ? q.ctas : q.units, sets = q.samples ? q.ctas : (size_t)B * q.sets;
+  l.part = take(sizeof(double2) * (size_t)G * std::max<size_t>(rows, q.slots));
+  l.set_part = take(sizeof(double2) * (size_t)(backward ? C : G) * sets);
   if (backward) {
-    l.bpart = take(sizeof(float2) * (size_t)C * q.units);
-    l.sums = take(sizeof(double2) * (size_t)C * std::max(B, q.ctas * q.teams));
-    l.coef = take(sizeof(float4) * (size_t)B * G);
+    l.bpart = take(sizeof(float2) * (size_t)C * rows);
+    l.sums = take(sizeof(double2) * (size_t)C *
+                  (q.samples ? q.ctas : std::max(B, q.ctas * q.teams)));
+    l.coef = take(sizeof(float4) * (size_t)G * (q.samples ? q.ctas : B));
   }
   l.total = at;
   return l;
@@ -513,19 +532,17 @@ Layout layout(const Plan& q, int B, int C, int G, bool backward) {
 
 template <typename T, int V, bool DROP>
 bool launch_kernel(const NormArgs& p, bool backward, bool samples, cudaStream_t s) {
-  const unsigned slots = (unsigned)(device_sms() * kOcc);
+  const int grid = samples ? p.ctas : (int)std::min<unsigned>(p.tickets, device_sms() * kOcc);
   if (samples) {
-    const unsigned grid = std::min<unsigned>((unsigned)p.B, slots);
     if (backward) norm_backward_samples<T, V, DROP><<<grid, kT, 0, s>>>(p);
     else norm_forward_samples<T, V, DROP><<<grid, kT, 0, s>>>(p);
   } else {
-    const unsigned grid = std::min<unsigned>(p.tickets, slots);
     if (backward) norm_backward_kernel<T, V, DROP><<<grid, kT, 0, s>>>(p);
     else norm_forward_kernel<T, V, DROP><<<grid, kT, 0, s>>>(p);
   }
   count_launch();
   if (!check_launch(backward ? "group norm backward" : "group norm")) return false;
-  return !(samples && backward && p.B > 1) || launch_params<T>(p, p.B, s);
+  return !(samples && backward && grid > 1) || launch_params<T>(p, grid, s);
 }
 
 template <typename T, int V>

@@ -67,10 +67,11 @@ struct NormArgs {
   uint32_t* done;       // [B, sets] finished first-pass slices of a set
   uint32_t* sets_done;  // [B] finished sets
   uint32_t* ready;      // [B] 1: statistics (backward: coef) are there
+  // (the plain kernels' rows; the others have a row per slot or CTA)
   double2* part;        // forward: [B, slices, G] (sum x, sum x^2); streamed: [slots, G]
   float2* bpart;        // backward: [B, slices, C] (sum dz, sum dz (x - mu))
   double2* set_part;    // [B, sets, G (backward: C)] sums of a set's slices
-  double2* sums;        // backward: [B, C] (A, X); streamed: [CTAs, C]
+  double2* sums;        // backward: [B, C] (A, X); otherwise a CTA's sum of them, [CTAs, C]
   float4* coef;         // backward: [B, G] (mu, k2, k3, 0): dx = gamma r dz + k2 (x - mu) + k3
   void* dweight;        // [C] or null
   void* dbias;
@@ -257,10 +258,9 @@ __device__ bool finish_slice(const NormArgs& p, int b, int j, const P* part, int
 }
 
 // (A, X) of a channel from the sums centred on mu rounded to float32.
-__device__ __forceinline__ void finish_channel(const NormArgs& p, int b, int c, double2 v) {
+__device__ __forceinline__ double2 finish_channel(const NormArgs& p, int b, int c, double2 v) {
   const double2 st = __ldg(p.stats + (long long)b * p.G + c / p.Cg);
-  p.sums[(long long)b * p.C + c] =
-      make_double2(v.x, st.y * (v.y - (st.x - (double)(float)st.x) * v.x));
+  return make_double2(v.x, st.y * (v.y - (st.x - (double)(float)st.x) * v.x));
 }
 
 // dx = gamma r dz - r m1 - r^2 m2 (x - mu) with mu = muh + mul, from a group's
@@ -272,11 +272,10 @@ __device__ __forceinline__ float4 finish_coef(const NormArgs& p, double2 st, dou
   return make_float4((float)st.x, (float)k2, (float)(-st.y * v.x * inv - k2 * mul), 0.f);
 }
 
-// dx's coefficients of a sample whose sums this CTA has just written.
+// dx's coefficients [G] of a sample whose channel sums [C] this CTA has just written.
 template <typename T>
-__device__ void finish_coef(const NormArgs& p, int b) {
+__device__ void finish_coef(const NormArgs& p, int b, const double2* sums, float4* coef) {
   const double2* stats = p.stats + (long long)b * p.G;
-  const double2* sums = p.sums + (long long)b * p.C;
   __threadfence_block();
   cta_sync();
   const double inv = 1.0 / ((double)p.S * p.Cg);
@@ -300,7 +299,7 @@ __device__ void finish_coef(const NormArgs& p, int b) {
       // dx = gamma r dz - r m1 - r^2 m2 (x - mu), mu = muh + mul
       const double k2 = -st.y * st.y * v.y * inv;
       const double k3 = -st.y * v.x * inv - k2 * (st.x - (double)(float)st.x);
-      p.coef[(long long)b * p.G + g] = make_float4((float)st.x, (float)k2, (float)k3, 0.f);
+      coef[g] = make_float4((float)st.x, (float)k2, (float)k3, 0.f);
     }
   }
 }

@@ -162,10 +162,12 @@ def test_c_workspace_sizes(lib):
     assert size(0, 4, 8, 2, _lib.F16, False) == 0
     assert size(1, 4, 8, 3, _lib.F16, False) == 0
     assert size(1, 4, 8, 2, 7, False) == 0
-    for b, rows, c, g in ((1, 1, 1, 1), (8, 32400, 256, 32), (1000, 3, 96, 96)):
+    for b, rows, c, g in ((1, 1, 1, 1), (8, 32400, 256, 32), (3, 4000, 33, 11)):
         fwd, bwd = (size(b, rows, c, g, _lib.F16, back) for back in (False, True))
         # a pair of float64 per sample, slice and group; of float32 per channel
         assert fwd >= 4 * (b + 1) + 16 * b * g
         assert bwd >= 4 * (b + 1) + 8 * b * c + 16 * b * c + 16 * b * g
     assert ctypes.sizeof(ctypes.c_size_t) == 8
+    # a million samples of one row: rows for the CTAs, not for the samples
+    assert size(1 << 20, 1, 256, 32, _lib.F16, True) < 32 << 20
     assert size(64, 1 << 20, 64, 8, _lib.F16, True) < 1 << 30
