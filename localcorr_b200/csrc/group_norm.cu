@@ -476,13 +476,13 @@ Plan make_plan(int B, long long S, int C, int dtype, bool backward) {
   q.lag = (uint32_t)std::min<long long>(
       units, slices + (long long)((32 << 20) / (maps * q.slice_rows * C * es)));
   // streamed kernels: up to 16 MB one chunk for both teams together, else an even number
-  // of chunks of up to 160 MB. Smaller chunks would be read a second time out of L2
-  // altogether (33 MB: 141 of 133 MB from HBM, 66 MB: 183), but each exchange of sums
-  // costs more than that saves: 8 x 135 x 240 x 256 float16 takes forward 77, 71 and 71 us
-  // and backward 155, 132 and 120 us in chunks of at most 30, 72 and 160 MB
-  const double total = maps * (double)S * B * C * es;
+  // of chunks of up to 72 MB, backward 160 MB. Smaller ones would be read a second time
+  // out of L2 altogether, but each exchange of sums costs more than that saves. In chunks
+  // of 33, 66 and 133 MB 8 x 135 x 240 x 256 float16 takes 74, 72 and 72 us forward, 142,
+  // 129 and 119 us backward; 8 x 540 x 960 x 64 in chunks of 66 and 133 MB 254 and 264 us
+  const double total = maps * (double)S * B * C * es, target = (backward ? 160 : 72) << 20;
   const long long k = std::min<long long>(
-      B, total < (16 << 20) ? 1 : 2 * (long long)(total / (2.0 * (160 << 20))) + 2);
+      B, total < (16 << 20) ? 1 : 2 * (long long)(total / (2 * target)) + 2);
   q.chunk = (int)((B + k - 1) / k);
   q.chunks = (B + q.chunk - 1) / q.chunk;
   q.teams = q.chunks > 1 ? 2 : 1;

@@ -8,14 +8,14 @@
 // ring of stages with bulk copies, running on across passes; the other warps do the
 // arithmetic, two float32 operations an instruction.
 //
-// Between the passes the team's CTAs wait for each other's sums, 5 to 6 us. So there are
+// Between the passes the team's CTAs wait for each other's sums, about 5 us. So there are
 // two teams, one CTA of each on every multiprocessor, that take the chunks in turn: while
 // one waits, the other streams, and reads of one overlap writes of the other.
 //
 // The sums travel through 16-byte entries that are written whole and start out as all
 // ones: a reader polls the entry itself, so no fence, counter or flag stands between a
-// sum and its reader, and every CTA adds up the entries of its samples itself, one
-// round trip after the last of them is written. Waiting needs every CTA resident: the
+// sum and its reader, and every CTA adds up the entries of its samples itself, two
+// round trips after the last of them is written. Waiting needs every CTA resident: the
 // kernels are launched cooperatively. (Dynamic units finished by the last arriver of
 // an atomic counter made the statistics wait 13 to 18 us: a round trip takes 2 to 3 us
 // while the copies saturate HBM.)
@@ -329,36 +329,57 @@ __device__ __forceinline__ Entry poll(const void* p, volatile int* abort) {
       atomicExch(&norm_status, 1);
       return Entry{0, 0};
     }
-    __nanosleep(40);
+    __nanosleep(200);
   }
 }
 // done(g, sum of the sample's entries of group g) by one thread per group, in an order
-// that only the sizes decide. All arithmetic threads take part, `width` of them a
-// group, with up to kFlight entries each in flight.
+// that only the sizes decide; `red` is room for kS double2. The entries of a sample lie
+// together, [runs, G]: a warp reads lines of them whole (one group's entries a warp at
+// a time, 32 lines a load, kept L2 busy for longer than the map's own rows).
 template <typename F>
 __device__ __forceinline__ void sample_sums(const NormArgs& p, int b, volatile int* abort,
-                                            F done) {
-  constexpr int kFlight = 8;
+                                            double2* red, F done) {
+  constexpr int kFlight = 5, kWarps = kS / 32;
   const Chunk c(p, b / p.chunk);
   const int s = b - c.first;
   const int first = c.run_of(s * p.S), runs = c.run_of((s + 1) * p.S - 1) - first + 1;
-  const int width = p.G >= kS ? 1 : min(32, pow2_below(kS / p.G));
-  const int lane = threadIdx.x % width;
-  for (int g0 = 0; g0 < p.G; g0 += kS / width) {
-    const int g = g0 + threadIdx.x / width;
+  const double2* part = p.part + (c.slots + first + s) * p.G;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  // One warp waits for the runs, by their first group, so that the others do not flood L2
+  // with polls meanwhile: 66 MB chunks took 64 us with all polling and 41 with one warp.
+  if (warp == 0) {
+#pragma unroll 1
+    for (int at = lane; at < runs; at += kFlight * 32) {
+      Entry e[kFlight];
+#pragma unroll
+      for (int u = 0; u < kFlight; ++u)  // past the end: the last one again
+        e[u] = get(part + (long long)min(at + u * 32, runs - 1) * p.G);
+#pragma unroll
+      for (int u = 0; u < kFlight; ++u)
+        if (!e[u].ready()) poll(part + (long long)min(at + u * 32, runs - 1) * p.G, abort);
+    }
+  }
+  stream_sync();
+  // a block of `wide` groups by `team` warps, 32 / wide runs a warp at a time
+  const int wide = p.G >= 32 ? 32 : p.G <= 1 ? 1 : 2 * pow2_below(p.G - 1);
+  const int blocks = (p.G + wide - 1) / wide, rows = 32 / wide;
+  const int team = blocks >= kWarps ? 1 : kWarps / (blocks <= 1 ? 1 : 2 * pow2_below(blocks - 1));
+  for (int k0 = 0; k0 < blocks; k0 += kWarps / team) {
+    const int k = k0 + warp / team, g = k * wide + lane % wide;
     double2 v = make_double2(0.0, 0.0);
     if (g < p.G) {
-      const double2* src = p.part + (c.slots + first + s) * p.G + g;
+      const double2* src = part + g;
+      const int step = team * rows;
 #pragma unroll 1
-      for (int at = lane; at < runs; at += kFlight * width) {
+      for (int at = warp % team * rows + lane / wide; at < runs; at += kFlight * step) {
         Entry e[kFlight];
 #pragma unroll
-        for (int u = 0; u < kFlight; ++u)  // past the end: the last one again
-          e[u] = get(src + (long long)min(at + u * width, runs - 1) * p.G);
+        for (int u = 0; u < kFlight; ++u)
+          e[u] = get(src + (long long)min(at + u * step, runs - 1) * p.G);
 #pragma unroll
         for (int u = 0; u < kFlight; ++u) {
-          if (at + u * width < runs) {
-            if (!e[u].ready()) e[u] = poll(src + (long long)(at + u * width) * p.G, abort);
+          if (at + u * step < runs) {
+            if (!e[u].ready()) e[u] = poll(src + (long long)(at + u * step) * p.G, abort);
             const double2 d = pair_of(e[u]);
             v.x += d.x;
             v.y += d.y;
@@ -366,8 +387,21 @@ __device__ __forceinline__ void sample_sums(const NormArgs& p, int b, volatile i
         }
       }
     }
-    v = lanes_sum(v, width);
-    if (g < p.G && lane == 0) done(g, v);
+    for (int o = wide; o < 32; o *= 2) {
+      v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
+      v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
+    }
+    if (team > 1) {
+      red[threadIdx.x] = v;
+      stream_sync();
+      if (warp % team == 0)
+        for (int w = 1; w < team; ++w) {
+          v.x += red[threadIdx.x + 32 * w].x;
+          v.y += red[threadIdx.x + 32 * w].y;
+        }
+      stream_sync();
+    }
+    if (g < p.G && warp % team == 0 && lane < wide) done(g, v);
   }
 }
 
@@ -437,12 +471,12 @@ __device__ __forceinline__ bool stats_unit(const NormArgs& p, const Place& at, C
 
 template <typename T, bool WHOLE, bool DROP, typename C>
 __device__ __forceinline__ bool apply_unit(const NormArgs& p, const Place& at, C& in,
-                                           double2* stats) {
+                                           double2* red, double2* stats) {
   constexpr int V = 16 / sizeof(T), N = WHOLE ? 1 : V / 2;
   const int b = in.now.b, c0 = at.col * V;
   const bool top = in.now.flags & kTop;
   stream_sync();  // the last sample's have been read
-  sample_sums(p, b, &in.r.abort, [&](int g, double2 t) {
+  sample_sums(p, b, &in.r.abort, red, [&](int g, double2 t) {
     stats[g] = finish_stats(p, t);
     if (top) p.stats[(long long)b * p.G + g] = stats[g];
   });
@@ -535,7 +569,7 @@ __global__ void __launch_bounds__(kBlock, kPerSm) norm_forward_stream(NormArgs p
   const Place at(p.C / (16 / (int)sizeof(T)), 0, kS);
   Consumer<1, ForwardShared<T, WHOLE>::kStages> in(sh.ring);
   while (in.open()) {
-    if (in.now.flags & kSecond ? !apply_unit<T, WHOLE, DROP>(p, at, in, sh.stats)
+    if (in.now.flags & kSecond ? !apply_unit<T, WHOLE, DROP>(p, at, in, sh.sums, sh.stats)
                                : !stats_unit<T, WHOLE>(p, at, in, sh))
       break;
   }
@@ -548,7 +582,7 @@ template <typename T, bool WHOLE>
 struct BackwardShared {
   static constexpr int kV = 16 / sizeof(T), kStages = 5;
   RingShared<2, kStages> ring;
-  float2 sums[kS * kV];  // sum dz, sum dz (x - mu)
+  alignas(16) float2 sums[kS * kV];  // sum dz, sum dz (x - mu); also kS double2
   float4 coef[1];        // [G] of the second pass's sample
 };
 
@@ -717,11 +751,11 @@ __device__ __forceinline__ bool grad_sums_unit(const NormArgs& p, const Place& a
 
 template <typename T, bool WHOLE, bool RECT, bool DROP, typename C>
 __device__ __forceinline__ bool grad_input_unit(const NormArgs& p, const Place& at, C& in,
-                                                float4* coef) {
+                                                double2* red, float4* coef) {
   constexpr int V = 16 / sizeof(T), N = WHOLE ? 1 : V / 2;
   const int b = in.now.b, c0 = at.col * V;
   stream_sync();  // the last sample's have been read
-  sample_sums(p, b, &in.r.abort, [&](int g, double2 t) {
+  sample_sums(p, b, &in.r.abort, red, [&](int g, double2 t) {
     coef[g] = finish_coef(p, __ldg(p.stats + (long long)b * p.G + g), t);
   });
   stream_sync();
@@ -771,7 +805,8 @@ __global__ void __launch_bounds__(kBlock, kPerSm) norm_backward_stream(NormArgs 
   bool started = false;  // whether this CTA's row of parameter sums holds something
   while (in.open()) {
     if (in.now.flags & kSecond
-            ? !grad_input_unit<T, WHOLE, RECT, DROP>(p, at, in, sh.coef)
+            ? !grad_input_unit<T, WHOLE, RECT, DROP>(p, at, in, reinterpret_cast<double2*>(sh.sums),
+                                                            sh.coef)
             : !grad_sums_unit<T, WHOLE, RECT, DROP>(p, at, in, sh.sums, &started))
       break;
   }
