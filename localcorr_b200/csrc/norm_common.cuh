@@ -120,13 +120,6 @@ __device__ __forceinline__ float act_value(float z, int act, float slope) {
   return z;
 }
 
-template <int V>
-__device__ __forceinline__ void act_values(float (&z)[V], int act, float slope) {
-  if (act == LCB200_ACT_NONE) return;
-#pragma unroll
-  for (int v = 0; v < V; ++v) z[v] = act_value(z[v], act, slope);
-}
-
 __device__ __forceinline__ float act_grad(float z, float g, int act, float slope) {
   if (act == LCB200_ACT_SILU) {
     const float sg = sigmoid(z);

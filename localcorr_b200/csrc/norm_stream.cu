@@ -154,7 +154,6 @@ struct StageInfo {
   int rows;       // of the stage
   int b;          // sample
   int seg;        // slot of the segment's sums
-  int seg_rows;
   int flags;
 };
 enum : int { kSecond = 1, kLast = 2, kEnd = 4, kTop = 8 };  // kTop: starts the sample
@@ -242,8 +241,8 @@ __device__ void produce(const NormArgs& p, RingShared<NM, STAGES>& r, const T* m
     const uint64_t policy = second ? go : stay;
     // a second pass runs backwards: what was read last is what L2 still holds
     each_segment(p, c.start(q), c.start(q + 1), second, [&](int s, long long r0, long long r1) {
-      const int seg = (int)(c.slots + q + s), seg_rows = (int)(r1 - r0);
-      const int stages = (seg_rows + p.stage_rows - 1) / p.stage_rows;
+      const int seg = (int)(c.slots + q + s);
+      const int stages = (int)((r1 - r0 + p.stage_rows - 1) / p.stage_rows);
       const int flags = (second ? kSecond : 0) | (r0 == 0 ? kTop : 0);
       for (int t = 0; t < stages && good && (good = claim()); ++t) {
         const int at = n % STAGES;
@@ -251,8 +250,8 @@ __device__ void produce(const NormArgs& p, RingShared<NM, STAGES>& r, const T* m
         const int rows = (int)min((long long)p.stage_rows, r1 - row);
         const uint32_t bytes = (uint32_t)(rows * p.C * sizeof(T));
         const long long off = ((long long)(c.first + s) * p.S + row) * p.C;
-        r.info[at] = StageInfo{off, rows, c.first + s, seg, seg_rows,
-                               flags | (t == stages - 1 ? kLast : 0)};
+        r.info[at] =
+            StageInfo{off, rows, c.first + s, seg, flags | (t == stages - 1 ? kLast : 0)};
         tc::mbar_arrive_expect_tx(&r.full[at], bytes * NM);
         bulk_copy(r.data[at][0], m0 + off, bytes, &r.full[at], policy);
         if (NM > 1) bulk_copy(r.data[at][NM - 1], m1 + off, bytes, &r.full[at], policy);
@@ -332,6 +331,7 @@ __device__ __forceinline__ Entry poll(const void* p, volatile int* abort) {
     __nanosleep(200);
   }
 }
+
 // done(g, sum of the sample's entries of group g) by one thread per group, in an order
 // that only the sizes decide; `red` is room for kS double2. The entries of a sample lie
 // together, [runs, G]: a warp reads lines of them whole (one group's entries a warp at
@@ -346,7 +346,8 @@ __device__ __forceinline__ void sample_sums(const NormArgs& p, int b, volatile i
   const double2* part = p.part + (c.slots + first + s) * p.G;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   // One warp waits for the runs, by their first group, so that the others do not flood L2
-  // with polls meanwhile: 66 MB chunks took 64 us with all polling and 41 with one warp.
+  // with polls meanwhile: a 66 MB chunk took 64 us with all polling, 41 with one warp, and
+  // 35 once the entries were read in whole lines.
   if (warp == 0) {
 #pragma unroll 1
     for (int at = lane; at < runs; at += kFlight * 32) {
@@ -583,7 +584,7 @@ struct BackwardShared {
   static constexpr int kV = 16 / sizeof(T), kStages = 5;
   RingShared<2, kStages> ring;
   alignas(16) float2 sums[kS * kV];  // sum dz, sum dz (x - mu); also kS double2
-  float4 coef[1];        // [G] of the second pass's sample
+  float4 coef[1];                    // [G] of the second pass's sample
 };
 
 // What z of a thread's channels takes, and dz in place of the output gradient.
@@ -644,16 +645,18 @@ struct Slope {
       }
     }
     if (RECT) {
-      const float slope = p.act == LCB200_ACT_RELU ? 0.f : p.slope;
+      auto side = [&](auto closed) {  // closed(v): what stays of g[v] below the corner
 #pragma unroll
-      for (int v = 0; v < V / 2; ++v) {
-        const float2 z =
-            add2(fma2(d[v], a[v], b[v]), fma2(d[v], al[v % H], bl[v % H]));
-        const float2 low = mul2(g[v], twice(slope));
-        g[v].x = z.x > 0.f ? g[v].x : low.x;
-        g[v].y = z.y > 0.f ? g[v].y : low.y;
-        d[v] = add2(d[v], mu[WHOLE ? 0 : v % N]);
-      }
+        for (int v = 0; v < V / 2; ++v) {
+          const float2 z = add2(fma2(d[v], a[v], b[v]), fma2(d[v], al[v % H], bl[v % H]));
+          const float2 low = closed(v);
+          g[v].x = z.x > 0.f ? g[v].x : low.x;
+          g[v].y = z.y > 0.f ? g[v].y : low.y;
+          d[v] = add2(d[v], mu[WHOLE ? 0 : v % N]);
+        }
+      };
+      if (p.act == LCB200_ACT_RELU) side([&](int) { return twice(0.f); });
+      else side([&](int v) { return mul2(g[v], twice(p.slope)); });
     } else {
 #pragma unroll
       for (int v = 0; v < V / 2; ++v) d[v] = add2(d[v], mu[WHOLE ? 0 : v % N]);

@@ -241,6 +241,20 @@ def test_norm_statistics_are_float64(rows):
                                atol=0)
 
 
+@pytest.mark.parametrize("shape", [(1, 20, 64), (2, 2000, 64), (2, 3000, 33)])
+def test_relu_gradient_of_what_is_not_finite(shape):
+    # an infinite output gradient behind a closed rectifier does not reach the bias
+    x, w, b, dy = (t.to(DEV) for t in _norm_case(shape, torch.float32, seed=41))
+    gb = b.clone().requires_grad_(True)
+    y = lc.group_norm(x, 1, w, gb, activation="relu")
+    closed = y.detach() == 0
+    assert bool(closed.any())
+    (g,) = torch.autograd.grad(y, gb, torch.where(closed, float("inf"), dy))
+    (want,) = torch.autograd.grad(lc.group_norm(x, 1, w, gb, activation="relu"), gb,
+                                  torch.where(closed, 0.0, dy))
+    assert torch.equal(g, want)
+
+
 def test_norm_large_float16_values():
     # squares far beyond float16's range
     x, w, b, dy = _norm_case((1, 100, 16), torch.float32, seed=8)
