@@ -135,6 +135,8 @@ def _check_norm(x, w, b, dy, groups, act, p=0.0, stream=(7, 3), mode="element", 
     ((3, 65, 1032), 3),        # rows no thread tiling fits evenly
     ((2, 150, 512), 512),      # the most groups that are streamed
     ((2, 150, 520), 520),      # one vector more
+    ((3, 50, 1), 1),           # a single channel
+    ((2, 90000, 1), 1),        # the same, divided
 ])
 def test_norm_against_oracle(dtype, act, shape, groups):
     x, w, b, dy = _norm_case(shape, DTYPES[dtype])
@@ -599,6 +601,30 @@ def test_compiled_step_equals_eager():
                     torch.autograd.grad(got, (x, w, b), dy)):
         # the residual's and the dropout's gradients may be added in another order
         torch.testing.assert_close(a, o, rtol=2.0 ** -9, atol=2.0 ** -9)
+
+
+def test_parameters_of_other_strides_and_shared_leaves():
+    x, w, b, dy = (t.to(DEV) for t in _norm_case((2, 30, 40), torch.float16))
+    one = torch.full((1,), 1.25, device=DEV, requires_grad=True)
+    pair = torch.stack([w, b], dim=1).requires_grad_(True)      # columns: stride 2
+    y = lc.group_norm(x, 5, one.expand(40), None, activation="silu")
+    (g,) = torch.autograd.grad(y, one, dy)
+    full = torch.full((40,), 1.25, device=DEV, requires_grad=True)
+    (want,) = torch.autograd.grad(lc.group_norm(x, 5, full, None, activation="silu"), full, dy)
+    torch.testing.assert_close(g, want.sum(0, keepdim=True))
+    (gp,) = torch.autograd.grad(lc.group_norm(x, 5, pair[:, 0], pair[:, 1]), pair, dy)
+    lw, lb = w.clone().requires_grad_(True), b.clone().requires_grad_(True)
+    gw, gb = torch.autograd.grad(lc.group_norm(x, 5, lw, lb), (lw, lb), dy)
+    assert torch.equal(gp, torch.stack([gw, gb], dim=1))
+
+
+def test_same_graph_twice():
+    x, w, b, dy = (t.to(DEV) for t in _norm_case((2, 300, 64), torch.float16))
+    xg = x.requires_grad_(True)
+    y = lc.dropout(lc.group_norm(xg, 8, w, b, activation="relu", p=0.2, rng=(1, 2)), 0.5, (1, 3))
+    first, = torch.autograd.grad(y, xg, dy, retain_graph=True)
+    again, = torch.autograd.grad(y, xg, dy)
+    assert torch.equal(first, again)
 
 
 def test_refusals():
