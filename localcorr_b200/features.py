@@ -110,6 +110,39 @@ def _check_norm(x, num_groups, weight, bias, eps, activation, negative_slope):
         raise ValueError(f"{what}: negative_slope must be finite, but got {negative_slope}")
 
 
+def _check_residual(x, residual):
+    if residual is None:
+        return
+    _check_map(residual, "dropout", "residual")
+    if residual.shape != x.shape or residual.dtype != x.dtype or residual.device != x.device:
+        raise ValueError(
+            f"dropout: the residual must be like x, {x.dtype} {tuple(x.shape)} on {x.device}, "
+            f"but got {residual.dtype} {tuple(residual.shape)} on {residual.device}")
+
+
+def _check_used(used, p, grad, what):
+    """The stream a forward left for its backward; one with p = 0 may leave none."""
+    if used is None or used.numel() == 0:
+        if p > 0:
+            raise ValueError(f"{what}: dropout with p > 0 needs the stream that the forward used")
+        return
+    _check_dropout(p, used, "element", grad, what)
+    if not used.is_contiguous():
+        raise ValueError(f"{what}: the stream used must be contiguous")
+
+
+def _check_norm_backward(grad_y, x, stats, num_groups):
+    what = "group_norm backward"
+    if grad_y.shape != x.shape or grad_y.device != x.device:
+        raise ValueError(f"{what}: the output gradient must be like x, {tuple(x.shape)} on "
+                         f"{x.device}, but got {tuple(grad_y.shape)} on {grad_y.device}")
+    if (stats.shape != (x.shape[0], num_groups, 2) or stats.dtype != torch.float64
+            or stats.device != x.device or not stats.is_contiguous()):
+        raise ValueError(f"{what}: the statistics must be the forward's, float64 "
+                         f"{(x.shape[0], num_groups, 2)} on {x.device}, but got {stats.dtype} "
+                         f"{tuple(stats.shape)} on {stats.device}")
+
+
 # ---------------------------------------------------------------------------
 # raw launchers (no autograd)
 # ---------------------------------------------------------------------------
@@ -332,12 +365,7 @@ def dropout(x, p, rng, residual=None, mode="element"):
     """
     _check_map(x, "dropout")
     p = _check_dropout(p, rng, mode, x, "dropout")
-    if residual is not None:
-        _check_map(residual, "dropout", "residual")
-        if residual.shape != x.shape or residual.dtype != x.dtype or residual.device != x.device:
-            raise ValueError(
-                f"dropout: the residual must be like x, {x.dtype} {tuple(x.shape)} on {x.device}, "
-                f"but got {residual.dtype} {tuple(residual.shape)} on {residual.device}")
+    _check_residual(x, residual)
     tensor, seed, offset = _split_rng(rng)
     args = (x, residual, p, mode == "channel", tensor, seed, offset)
     if torch.compiler.is_compiling():

@@ -236,13 +236,21 @@ spatial_corr.register_autograd(_sc_backward, setup_context=_sc_setup)
 
 
 # ---------------------------------------------------------------------------
-# feature-map operators
+# feature-map operators. They check their arguments as the public functions do: a
+# direct call reaches them without those.
 # ---------------------------------------------------------------------------
+
+def _rng_argument(rng, seed, offset):
+    return rng if rng is not None else (seed, offset)
+
 
 @custom_op(f"{_NS}::group_norm", mutates_args=(), device_types="cuda")
 def group_norm(x: Tensor, weight: Optional[Tensor], bias: Optional[Tensor], num_groups: int,
                eps: float, activation: str, negative_slope: float, p: float, channel: bool,
                rng: Optional[Tensor], seed: int, offset: int) -> tuple[Tensor, Tensor, Tensor]:
+    features._check_map(x, "group_norm")
+    features._check_norm(x, num_groups, weight, bias, eps, activation, negative_slope)
+    features._check_dropout(p, _rng_argument(rng, seed, offset), "element", x, "group_norm")
     y, stats, used = features.group_norm_forward(x, weight, bias, num_groups, eps, activation,
                                                  negative_slope, p, channel, rng, seed, offset)
     return y, stats, used if used is not None else x.new_empty((0,), dtype=torch.int64)
@@ -265,6 +273,10 @@ def group_norm_backward(grad_y: Tensor, x: Tensor, weight: Optional[Tensor],
                         activation: str, negative_slope: float, p: float,
                         channel: bool) -> tuple[Tensor, Tensor, Tensor]:
     """Gradients of x, weight and bias (empty for an absent parameter)."""
+    features._check_map(x, "group_norm backward")
+    features._check_norm(x, num_groups, weight, bias, 0.0, activation, negative_slope)
+    features._check_norm_backward(grad_y, x, stats, num_groups)
+    features._check_used(used, p, x, "group_norm backward")
     gx, gw, gb = features.group_norm_backward(grad_y, x, weight, bias, stats, used, num_groups,
                                               activation, negative_slope, p, channel)
     return gx, gw if gw is not None else _absent(x), gb if gb is not None else _absent(x)
@@ -298,6 +310,9 @@ group_norm.register_autograd(_gn_backward, setup_context=_gn_setup)
 @custom_op(f"{_NS}::dropout", mutates_args=(), device_types="cuda")
 def dropout(x: Tensor, residual: Optional[Tensor], p: float, channel: bool,
             rng: Optional[Tensor], seed: int, offset: int) -> tuple[Tensor, Tensor]:
+    features._check_map(x, "dropout")
+    features._check_residual(x, residual)
+    features._check_dropout(p, _rng_argument(rng, seed, offset), "element", x, "dropout")
     return features.dropout_forward(x, residual, p, channel, rng, seed, offset)
 
 
@@ -308,6 +323,8 @@ def _(x, residual, p, channel, rng, seed, offset):
 
 @custom_op(f"{_NS}::dropout_backward", mutates_args=(), device_types="cuda")
 def dropout_backward(grad_y: Tensor, used: Tensor, p: float, channel: bool) -> Tensor:
+    features._check_map(grad_y, "dropout backward", "grad_y")
+    features._check_used(used, p, grad_y, "dropout backward")
     return features.dropout_backward(grad_y, used, p, channel)
 
 

@@ -171,3 +171,34 @@ def test_c_workspace_sizes(lib):
     # a million samples of one row: rows for the CTAs, not for the samples
     assert size(1 << 20, 1, 256, 32, _lib.F16, True) < 32 << 20
     assert size(64, 1 << 20, 64, 8, _lib.F16, True) < 1 << 30
+
+
+@pytest.mark.parametrize("kw,match", [
+    (dict(grad_y=torch.zeros(2, 5, 4)), "like x"),
+    (dict(grad_y=torch.zeros(1, 5, 8)), "like x"),
+    (dict(stats=torch.zeros(2, 4, 2)), "float64"),
+    (dict(stats=torch.zeros(2, 2, 2, dtype=torch.float64)), "statistics"),
+    (dict(stats=torch.zeros(1, 4, 2, dtype=torch.float64).expand(2, 4, 2)), "statistics"),
+])
+def test_norm_backward_arguments(kw, match):
+    args = dict(grad_y=torch.zeros(2, 5, 8), x=torch.zeros(2, 5, 8),
+                stats=torch.zeros(2, 4, 2, dtype=torch.float64), num_groups=4)
+    features._check_norm_backward(**args)
+    with pytest.raises(ValueError, match=match):
+        features._check_norm_backward(**{**args, **kw})
+
+
+@pytest.mark.parametrize("used,p,match", [
+    (None, 0.5, "needs the stream"),
+    (torch.zeros(0, dtype=torch.int64), 0.5, "needs the stream"),
+    (torch.zeros(3, dtype=torch.int64), 0.5, "rng tensor"),
+    (torch.zeros(2), 0.0, "rng tensor"),
+    (torch.zeros(2, 2, dtype=torch.int64)[:, 0], 0.5, "contiguous"),
+    (torch.zeros(2, dtype=torch.int64), 1.5, "probability"),
+])
+def test_used_stream_arguments(used, p, match):
+    x = torch.zeros(2, 5, 8)
+    features._check_used(None, 0.0, x, "backward")
+    features._check_used(torch.zeros(2, dtype=torch.int64), 0.5, x, "backward")
+    with pytest.raises(ValueError, match=match):
+        features._check_used(used, p, x, "backward")

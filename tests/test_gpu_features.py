@@ -652,6 +652,42 @@ def test_refusals():
         g.sum().backward()
 
 
+def test_registered_operators_refuse_what_the_functions_refuse():
+    op = torch.ops.localcorr
+    x = torch.zeros(2, 5, 8, device=DEV)
+    used = torch.zeros(2, dtype=torch.int64, device=DEV)
+    stats = torch.ones(2, 4, 2, dtype=torch.float64, device=DEV)
+
+    def norm(x=x, w=None, groups=4, act="relu", p=0.0, rng=None, seed=1):
+        return op.group_norm(x, w, None, groups, 1e-5, act, 0.0, p, False, rng, seed, 0)
+
+    def back(dy=x, w=None, stats=stats, used=used, p=0.0):
+        return op.group_norm_backward(dy, x, w, None, stats, used, 4, "relu", 0.0, p, False)
+
+    norm(), back(), back(used=None)
+    for call, err in [
+            (lambda: norm(w=torch.ones(7, device=DEV)), ValueError),
+            (lambda: norm(w=torch.ones(8)), RuntimeError),
+            (lambda: norm(x.double()), RuntimeError),
+            (lambda: norm(groups=3), ValueError),
+            (lambda: norm(act="gelu"), ValueError),
+            (lambda: norm(p=0.5, rng=used[:1]), ValueError),
+            (lambda: norm(p=0.5, rng=used.cpu()), ValueError),
+            (lambda: norm(p=0.5, seed=-1), ValueError),
+            (lambda: back(x[:1]), ValueError),
+            (lambda: back(w=torch.ones(7, device=DEV)), ValueError),
+            (lambda: back(stats=stats[:1]), ValueError),
+            (lambda: back(stats=stats.float()), ValueError),
+            (lambda: back(used=None, p=0.5), ValueError),
+            (lambda: op.dropout(x, x[:1], 0.5, False, None, 1, 2), ValueError),
+            (lambda: op.dropout(x, None, 0.5, False, used[:1], 0, 0), ValueError),
+            (lambda: op.dropout(x, None, 2.0, False, None, 1, 2), ValueError),
+            (lambda: op.dropout_backward(x, used[:1], 0.5, False), ValueError),
+            (lambda: op.dropout_backward(x.int(), used, 0.5, False), RuntimeError)]:
+        with pytest.raises(err):
+            call()
+
+
 def test_run_of_an_encoders_tail_into_the_correlation():
     """norm + ReLU + channel dropout on both maps, a dropped branch added to it, the pyramid
     lookup, and the gradients of everything, against the 64-bit oracle."""
