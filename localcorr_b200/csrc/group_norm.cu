@@ -26,9 +26,12 @@ __device__ void stats_slice(const NormArgs& p, int b, int j, double2* out, doubl
   for (int cb = 0; cb < cols; cb += kT) {
     const Place at(cols, cb);
     if (at.on) {
-      double s[V], q[V];
+      double s[V], q[V], k[V];
 #pragma unroll
-      for (int v = 0; v < V; ++v) s[v] = q[v] = 0.0;
+      for (int v = 0; v < V; ++v) {
+        s[v] = q[v] = 0.0;
+        k[v] = group_shift<T>(p, b, (at.col * V + v) / p.Cg);
+      }
       const T* ptr = xb + (long long)at.col * V;
       const long long step = at.rp;
       auto one = [&](typename Vec<T, V>::Raw raw) {
@@ -36,9 +39,9 @@ __device__ void stats_slice(const NormArgs& p, int b, int j, double2* out, doubl
         Vec<T, V>::unpack(raw, f);
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-          const double x = f[v];
-          s[v] += x;
-          q[v] = fma(x, x, q[v]);
+          const double d = (double)f[v] - k[v];
+          s[v] += d;
+          q[v] = fma(d, d, q[v]);
         }
       };
       long long r = r0 + at.row;
@@ -316,7 +319,7 @@ __global__ void __launch_bounds__(kT, kOcc) norm_forward_kernel(NormArgs p) {
     if (!second) {
       stats_slice<T, V>(p, b, j, p.part + ((long long)b * p.slices + j) * p.G, sm);
       if (finish_slice(p, b, j, p.part, p.G, sm, [&](int g, double2 t) {
-            p.stats[(long long)b * p.G + g] = finish_stats(p, t);
+            p.stats[(long long)b * p.G + g] = finish_stats(p, t, group_shift<T>(p, b, g));
           }))
         publish(p.ready + b);
       return true;
@@ -361,7 +364,7 @@ __global__ void __launch_bounds__(kT, kOcc) norm_forward_samples(NormArgs p) {
   for (int b = blockIdx.x; b < p.B; b += gridDim.x) {
     stats_slice<T, V>(p, b, 0, part, sm);
     for (int g = threadIdx.x; g < p.G; g += kT)
-      p.stats[(long long)b * p.G + g] = finish_stats(p, __ldcg(part + g));
+      p.stats[(long long)b * p.G + g] = finish_stats(p, __ldcg(part + g), group_shift<T>(p, b, g));
     cta_sync();
     apply_slice<T, V, DROP>(p, b, 0);
   }

@@ -13,12 +13,15 @@
 // needed before the first output, so a sample is read twice; see the launchers
 // for how the second read comes out of L2.
 //
-// Numerics. sum x and sum x^2 are float64 from the first addition on: every x and x^2
-// is exact there, and mean^2 / var can reach 1e8 before the cancellation in var costs
-// what float32 holds. (Float32 sums of (x - K)^2 over 110 rows left 1/std 1.7e-7 off for
-// bfloat16 maps: squares of odd integers are 1 modulo 8, so their roundings do not
-// average out.) That matters because a rectifier's gradient jumps at z = 0: with 1.7e-7,
-// one training step in three of a 67 million element map had elements on the wrong
+// Numerics. The sums are of x - K and (x - K)^2 with K the group's first value, float64
+// from the first addition on. K is one of the group's n values, so (mu - K)^2 is at most
+// (n - 1) var, and a few var for a map like any other, however far its mean lies from 0:
+// the cancellation in var = E[(x - K)^2] - (mu - K)^2 costs that factor of 2^-53 and no
+// more, and a constant group's var is 0 exactly. (Sums of x and x^2 left 1/std 3e-7 off
+// at mean / std = 1e5, 1e-4 off at 1e6. Float32 sums of (x - K)^2 over 110 rows left it
+// 1.7e-7 off for bfloat16 maps: squares of odd integers are 1 modulo 8, so their roundings
+// do not average out.) That matters because a rectifier's gradient jumps at z = 0: with
+// 1.7e-7, one training step in three of a 67 million element map had elements on the wrong
 // side. The backward therefore takes z = x a + b with a = gamma r, b = beta - mu a as
 // pairs of floats, whose sign is that of the float64 value but for ~2^-45.
 // The backward's own sums are float32 within a thread and float64 beyond. Partial sums
@@ -68,7 +71,7 @@ struct NormArgs {
   uint32_t* sets_done;  // [B] finished sets
   uint32_t* ready;      // [B] 1: statistics (backward: coef) are there
   // (the plain kernels' rows; the others have a row per slot or CTA)
-  double2* part;        // forward: [B, slices, G] (sum x, sum x^2); streamed: [slots, G]
+  double2* part;        // forward: [B, slices, G] (sum x - K, sum (x - K)^2); streamed: [slots, G]
   float2* bpart;        // backward: [B, slices, C] (sum dz, sum dz (x - mu))
   double2* set_part;    // [B, sets, G (backward: C)] sums of a set's slices
   double2* sums;        // backward: [B, C] (A, X); otherwise a CTA's sum of them, [CTAs, C]
@@ -176,13 +179,20 @@ __device__ __forceinline__ float affine_z(const Affine& f, float x) {
 }
 
 // ---- the end of a sample: statistics, or coefficients of dx --------------------
-// One group's mean and 1/std from its (sum x, sum x^2).
-__device__ __forceinline__ double2 finish_stats(const NormArgs& p, double2 v) {
+// The value K that a group's sums are centred on: its first.
+template <typename T>
+__device__ __forceinline__ double group_shift(const NormArgs& p, int b, int g) {
+  return (double)ldf(reinterpret_cast<const T*>(p.x) + (long long)b * p.S * p.C +
+                     (long long)g * p.Cg);
+}
+
+// One group's mean and 1/std from its (sum x - K, sum (x - K)^2).
+__device__ __forceinline__ double2 finish_stats(const NormArgs& p, double2 v, double shift) {
   const double inv = 1.0 / ((double)p.S * p.Cg);
   const double mean = v.x * inv;
   double var = v.y * inv - mean * mean;
   var = var < 0.0 ? 0.0 : var;  // rounding below zero; NaN stays
-  return make_double2(mean, 1.0 / sqrt(var + p.eps));
+  return make_double2(shift + mean, 1.0 / sqrt(var + p.eps));
 }
 
 // True in every thread of the CTA that finished last of `count` at *counter;

@@ -412,7 +412,7 @@ template <typename T, bool WHOLE>
 struct ForwardShared {
   static constexpr int kV = 16 / sizeof(T), kStages = WHOLE ? 5 : 4;
   RingShared<1, kStages> ring;
-  double2 sums[kS * (WHOLE ? 1 : kV)];  // (sum x, sum x^2) of each thread
+  double2 sums[kS * (WHOLE ? 1 : kV)];  // (sum x - K, sum (x - K)^2) of each thread
   double2 stats[1];                     // [G] of the second pass's sample
 };
 
@@ -420,9 +420,11 @@ template <typename T, bool WHOLE, typename C>
 __device__ __forceinline__ bool stats_unit(const NormArgs& p, const Place& at, C& in,
                                            ForwardShared<T, WHOLE>& sh) {
   constexpr int V = 16 / sizeof(T), N = WHOLE ? 1 : V, A = WHOLE ? 2 : V;
-  double s[A], q[A];
+  double s[A], q[A], k[N];
 #pragma unroll
   for (int v = 0; v < A; ++v) s[v] = q[v] = 0.0;
+#pragma unroll
+  for (int v = 0; v < N; ++v) k[v] = group_shift<T>(p, in.now.b, (at.col * V + v) / p.Cg);
   const int seg = in.now.seg;
   for (;;) {
     const uint4* data = in.map(0);
@@ -431,9 +433,9 @@ __device__ __forceinline__ bool stats_unit(const NormArgs& p, const Place& at, C
       Vec2<T>::unpack(data[i], f);
 #pragma unroll
       for (int v = 0; v < V; ++v) {
-        const double x = v & 1 ? f[v / 2].y : f[v / 2].x;
-        s[v % A] += x;
-        q[v % A] = fma(x, x, q[v % A]);
+        const double d = (double)(v & 1 ? f[v / 2].y : f[v / 2].x) - k[v % N];
+        s[v % A] += d;
+        q[v % A] = fma(d, d, q[v % A]);
       }
     });
     const bool last = in.now.flags & kLast;
@@ -477,8 +479,10 @@ __device__ __forceinline__ bool apply_unit(const NormArgs& p, const Place& at, C
   const int b = in.now.b, c0 = at.col * V;
   const bool top = in.now.flags & kTop;
   stream_sync();  // the last sample's have been read
+  // on their way while the sums are: sample_sums starts with a barrier
+  for (int g = threadIdx.x; g < p.G; g += kS) stats[g].x = group_shift<T>(p, b, g);
   sample_sums(p, b, &in.r.abort, red, [&](int g, double2 t) {
-    stats[g] = finish_stats(p, t);
+    stats[g] = finish_stats(p, t, stats[g].x);
     if (top) p.stats[(long long)b * p.G + g] = stats[g];
   });
   stream_sync();

@@ -1,0 +1,108 @@
+"""How exact the feature-map operators are, against 64-bit values on the GPU.
+
+Every tolerance is derived beside its use from the roundings the kernels make: float32's is
+2^-24, float64's 2^-53, relative to the rounded value.
+"""
+
+import pytest
+import torch
+
+import localcorr_b200 as lc
+from localcorr_b200 import _lib, features
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _need_gpu():
+    if not torch.cuda.is_available():
+        pytest.skip("CUDA device required")
+    assert _lib.load_library() is not None
+
+
+def _randn(shape, seed, dtype=torch.float64):
+    return torch.randn(shape, generator=torch.Generator(DEV).manual_seed(seed), device=DEV,
+                       dtype=dtype)
+
+
+def _by_group(x, groups):
+    return x.double().reshape(x.shape[0], -1, groups, x.shape[-1] // groups)
+
+
+def _statistics(x, groups, eps):
+    """Mean and 1/std [B, G] in float64, centred before they are squared."""
+    v = _by_group(x, groups)
+    mean = v.mean((1, 3), keepdim=True)
+    var = ((v - mean) ** 2).mean((1, 3), keepdim=True)
+    shape = (x.shape[0], groups)
+    return mean.reshape(shape), (1 / (var + eps).sqrt()).reshape(shape)
+
+
+def _kernel_statistics(x, groups, eps):
+    stats = features.group_norm_forward(x, None, None, groups, eps, "none", 0.0, 0.0, False, None,
+                                        0, 0)[1]
+    return stats[..., 0], stats[..., 1]
+
+
+# whole samples; streamed, groups of whole vectors and of single channels; plain, twice
+SIZES = [((2, 100, 64), 8), ((3, 4000, 64), 8), ((2, 2000, 64), 64), ((2, 3000, 33), 3),
+         ((1, 90, 4104), 8)]
+
+
+@pytest.mark.parametrize("eps", [1e-5, 0.0])
+@pytest.mark.parametrize("mean,std", [(0.0, 1.0), (1e4, 1.0), (1e5, 1.0), (1e6, 1.0),
+                                      (3000.0, 0.002), (-2e7, 10.0)])
+@pytest.mark.parametrize("shape,groups", SIZES)
+def test_statistics_of_maps_far_from_zero(shape, groups, mean, std, eps):
+    x = (_randn(shape, 1) * std + mean).float()
+    want_mean, want_rstd = _statistics(x, groups, eps)
+    got_mean, got_rstd = _kernel_statistics(x, groups, eps)
+    # float64 sums of at most 2^18 terms around a value of the group, which lies less than 6
+    # spreads from the mean: var is off by 37 * 2^18 * 2^-53 < 2^-29 of itself at the very worst
+    # (every rounding of one sign); 2^-34 allows for 2^13 of them, 1/std halves it
+    assert bool(((got_rstd - want_rstd).abs() <= 2.0 ** -35 * want_rstd).all())
+    assert bool(((got_mean - want_mean).abs()
+                 <= 2.0 ** -51 * abs(mean) + 2.0 ** -35 / want_rstd).all())
+
+
+@pytest.mark.parametrize("shape,groups", SIZES)
+def test_statistics_around_a_value_far_off(shape, groups):
+    # the first value of each group is 1000 spreads of the others away
+    x = _randn(shape, 2).float()
+    first = x.reshape(shape[0], -1, groups, shape[-1] // groups)
+    first[:, 0, :, 0] += 1000.0
+    want_mean, want_rstd = _statistics(x, groups, 1e-5)
+    got_mean, got_rstd = _kernel_statistics(x, groups, 1e-5)
+    # the cancellation costs (1000 spreads)^2 / var < 2^20 of 2^13 roundings of 2^-53
+    assert bool(((got_rstd - want_rstd).abs() <= 2.0 ** -20 * want_rstd).all())
+    assert bool(((got_mean - want_mean).abs() <= 2.0 ** -30).all())
+
+
+@pytest.mark.parametrize("shape,groups", SIZES)
+def test_small_variance_far_from_zero_without_eps(shape, groups):
+    # one value in a hundred is a float32 step (1/16) above 10^6
+    x = torch.full(shape, 1e6, device=DEV)
+    x.view(-1)[::99] += 0.0625
+    want_mean, want_rstd = _statistics(x, groups, 0.0)
+    # (33 channels in 3 groups: the values all lie in the first; a group without any has no
+    # variance, 1/std is infinite and the outputs are 0 / 0)
+    assert bool(want_rstd[:, 0].isfinite().all())
+    got_mean, got_rstd = _kernel_statistics(x, groups, 0.0)
+    # every x - K is a multiple of 1/16 and its sums are exact; the rest is a few roundings
+    torch.testing.assert_close(got_rstd, want_rstd, rtol=2.0 ** -45, atol=0)
+    y = lc.group_norm(x, groups, eps=0.0)
+    want = ((_by_group(x, groups) - want_mean[:, None, :, None])
+            * want_rstd[:, None, :, None]).reshape(shape)
+    # x - mu is exact but for mu's part below float32, whose product with 1/std (at most
+    # 1/30 * 10) is rounded; then 1/std, the product and the sum
+    assert torch.equal(y.isnan(), want.isnan())
+    off = ((y.double() - want).abs() - 2.0 ** -22 * (want.abs() + 1))[~want.isnan()]
+    assert bool((off <= 0).all())
+
+
+@pytest.mark.parametrize("shape,groups", SIZES)
+def test_constant_groups_give_the_bias(shape, groups):
+    x = torch.full(shape, 1234567.0, device=DEV)
+    b = torch.linspace(-1, 1, shape[-1], device=DEV)
+    assert torch.equal(lc.group_norm(x, groups, None, b), b.expand(shape))
