@@ -26,7 +26,7 @@ Operators (CUDA tensors only; all outputs are new tensors):
 * ``group_norm(x, weight, bias, num_groups, eps, activation, negative_slope, p,
   channel, rng, seed, offset)``: (dropout(act(group norm)) of a channels-last
   map, its statistics, the dropout stream used), see :mod:`localcorr_b200.features`.
-  Backward: ``group_norm_backward``.
+  Only the map is differentiable. Backward: ``group_norm_backward``.
 * ``dropout(x, residual, p, channel, rng, seed, offset)``: (residual +
   dropout(x), the stream used). Backward: ``dropout_backward``.
 """
@@ -292,6 +292,7 @@ def _(grad_y, x, weight, bias, stats, used, num_groups, activation, negative_slo
 def _gn_setup(ctx, inputs, output):
     x, weight, bias, num_groups, _, activation, slope, p, channel, _, _, _ = inputs
     _, stats, used = output
+    ctx.mark_non_differentiable(stats, used)  # a by-product: only y has a gradient formula
     ctx.save_for_backward(x, weight, bias, stats, used)
     ctx.params = (num_groups, activation, slope, p, channel)
 
@@ -335,6 +336,7 @@ def _(grad_y, used, p, channel):
 
 def _do_setup(ctx, inputs, output):
     _, residual, p, channel, _, _, _ = inputs
+    ctx.mark_non_differentiable(output[1])
     ctx.save_for_backward(output[1])
     ctx.params = (p, channel)
     ctx.residual = residual is not None

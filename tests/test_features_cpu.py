@@ -7,6 +7,7 @@ import ctypes
 import numpy as np
 import pytest
 import torch
+from torch._subclasses.fake_tensor import FakeTensorMode
 
 import localcorr_b200 as lc
 from localcorr_b200 import _lib, features
@@ -202,3 +203,15 @@ def test_used_stream_arguments(used, p, match):
     features._check_used(torch.zeros(2, dtype=torch.int64), 0.5, x, "backward")
     with pytest.raises(ValueError, match=match):
         features._check_used(used, p, x, "backward")
+
+
+def test_only_the_map_of_a_registered_operator_is_differentiable():
+    # the statistics have no gradient formula: a loss of them must not get a silent zero
+    with FakeTensorMode():
+        x = torch.empty(2, 5, 8, device="cuda", requires_grad=True)
+        w = torch.empty(8, device="cuda", requires_grad=True)
+        y, stats, used = torch.ops.localcorr.group_norm(x, w, None, 2, 1e-5, "relu", 0.0, 0.5,
+                                                        False, None, 1, 2)
+        assert y.requires_grad and not stats.requires_grad and not used.requires_grad
+        y, used = torch.ops.localcorr.dropout(x, x, 0.5, True, None, 1, 2)
+        assert y.requires_grad and not used.requires_grad

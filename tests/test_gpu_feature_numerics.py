@@ -106,3 +106,22 @@ def test_constant_groups_give_the_bias(shape, groups):
     x = torch.full(shape, 1234567.0, device=DEV)
     b = torch.linspace(-1, 1, shape[-1], device=DEV)
     assert torch.equal(lc.group_norm(x, groups, None, b), b.expand(shape))
+
+
+# ---------------------------------------------------------------------------
+# what autograd is told
+# ---------------------------------------------------------------------------
+
+def test_by_products_of_registered_operators_are_not_differentiable():
+    x = _randn((2, 30, 16), 3).float().requires_grad_(True)
+    w = torch.ones(16, device=DEV, requires_grad=True)
+    op = torch.ops.localcorr
+    y, stats, used = op.group_norm(x, w, None, 4, 1e-5, "silu", 0.0, 0.5, False, None, 1, 2)
+    assert not stats.requires_grad and not used.requires_grad
+    want = lc.group_norm(x, 4, w, activation="silu", p=0.5, rng=(1, 2))
+    for a, b in zip(torch.autograd.grad(y.sum(), (x, w)), torch.autograd.grad(want.sum(), (x, w))):
+        assert torch.equal(a, b)
+    with pytest.raises(RuntimeError, match="does not require grad"):
+        stats.sum().backward()
+    y, used = op.dropout(x, x, 0.5, True, None, 1, 2)
+    assert y.requires_grad and not used.requires_grad
