@@ -175,6 +175,7 @@ __device__ void grad_sums_slice(const NormArgs& p, int b, int j, float2* out, fl
     if (at.on) {
       Affine f[V];
       float mu[V], sa[V], sx[V];
+      double ta[V], tx[V];
       const int c0 = at.col * V;
 #pragma unroll
       for (int v = 0; v < V; ++v) {
@@ -182,7 +183,16 @@ __device__ void grad_sums_slice(const NormArgs& p, int b, int j, float2* out, fl
         f[v] = affine<T>(p, st, c0 + v);
         mu[v] = (float)st.x;
         sa[v] = sx[v] = 0.f;
+        ta[v] = tx[v] = 0.0;
       }
+      auto fold = [&]() {
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          ta[v] += sa[v];
+          tx[v] += sx[v];
+          sa[v] = sx[v] = 0.f;
+        }
+      };
       uint32_t keep = ~0u;
       if (DROP && p.drop.channel)
         keep = drop_keep<V>(ds, p.drop.threshold, (long long)b * p.C + c0);
@@ -204,7 +214,9 @@ __device__ void grad_sums_slice(const NormArgs& p, int b, int j, float2* out, fl
       long long r = r0 + at.row;
       const long long step = at.rp;
       constexpr int U = kUnroll / 2;
-      for (; r + (U - 1) * step < r1; r += U * step) {
+      // 16-byte vectors: 16 rows a thread at most, narrower ones up to 150
+      constexpr bool kFolds = V * sizeof(T) < 16;
+      for (int n = 1; r + (U - 1) * step < r1; r += U * step, ++n) {
         typename Vec<T, V>::Raw xr[U], gr[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
@@ -213,22 +225,24 @@ __device__ void grad_sums_slice(const NormArgs& p, int b, int j, float2* out, fl
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) one(xr[u], gr[u], r + u * step);
+        if (kFolds && n % (kRun / U) == 0) fold();
       }
       for (; r < r1; r += step)
         one(Vec<T, V>::load(xs + r * p.C), Vec<T, V>::load(gs + r * p.C), r);
+      fold();
 #pragma unroll
       for (int v = 0; v < V; ++v)
-        sm[(at.row * at.nc + (at.col - cb)) * V + v] = make_float2(sa[v], sx[v]);
+        sm[(at.row * at.nc + (at.col - cb)) * V + v] = make_float2((float)ta[v], (float)tx[v]);
     }
     __syncthreads();
     for (int i = threadIdx.x; i < at.nc * V; i += kT) {
-      float2 v = make_float2(0.f, 0.f);
+      double2 v = make_double2(0.0, 0.0);
       for (int k = 0; k < at.rp; ++k) {
         const float2 e = sm[k * at.nc * V + i];
         v.x += e.x;
         v.y += e.y;
       }
-      out[cb * V + i] = v;
+      out[cb * V + i] = make_float2((float)v.x, (float)v.y);
     }
     __syncthreads();
   }

@@ -24,9 +24,13 @@
 // 1.7e-7, one training step in three of a 67 million element map had elements on the wrong
 // side. The backward therefore takes z = x a + b with a = gamma r, b = beta - mu a as
 // pairs of floats, whose sign is that of the float64 value but for ~2^-45.
-// The backward's own sums are float32 within a thread and float64 beyond. Partial sums
-// have slots of their own and are added in a fixed order, with no float atomics: results
-// repeat bit for bit.
+// The backward's sums of dz and dz (x - mu) are float32 over at most kRun rows of a thread,
+// then over at most kRuns such sums, and float64 beyond; the plain kernels round a thread's
+// and a slice's sum to float32 once each. So n equal terms are off by 17 2^-24 a level at
+// most. (One float32 sum over a thread's rows left the gradient of a mean's bias 173 2^-24
+// off at 1024 rows a thread: equal terms round the same way until the sum doubles.)
+// Partial sums have slots of their own and are added in a fixed order, with no float
+// atomics: results repeat bit for bit.
 #pragma once
 
 #include "feature_common.cuh"
@@ -36,6 +40,8 @@ namespace lcb200 {
 constexpr int kT = 256;      // threads of a CTA
 constexpr int kOcc = 3;      // CTAs a multiprocessor holds
 constexpr int kUnroll = 4;   // rows a thread has in flight
+constexpr int kRun = 32;     // rows of a thread whose terms are added in float32
+constexpr int kRuns = 32;    // such sums added in float32
 constexpr long long kWaitLimit = 1 << 24;  // polls (100 ns and more each) before a wait gives up
 
 // 1: a wait ran out and a kernel of this translation unit stopped early

@@ -588,7 +588,7 @@ struct BackwardShared {
   static constexpr int kV = 16 / sizeof(T), kStages = 5;
   RingShared<2, kStages> ring;
   alignas(16) float2 sums[kS * kV];  // sum dz, sum dz (x - mu); also kS double2
-  float4 coef[1];                    // [G] of the second pass's sample
+  float4 coef[1];  // [G] of the second pass's sample; as double2 a first pass's group sums
 };
 
 // What z of a thread's channels takes, and dz in place of the output gradient.
@@ -677,57 +677,35 @@ struct Slope {
   }
 };
 
-template <typename T, bool WHOLE, bool RECT, bool DROP, typename C>
-__device__ __forceinline__ bool grad_sums_unit(const NormArgs& p, const Place& at, C& in,
-                                               float2* sums, bool* started) {
-  constexpr int V = 16 / sizeof(T);
-  const int b = in.now.b, seg = in.now.seg, c0 = at.col * V;
-  Slope<T, WHOLE, RECT, DROP> f(p, b, c0);
-  float2 sa[V / 2], sx[V / 2];
-#pragma unroll
-  for (int v = 0; v < V / 2; ++v) sa[v] = sx[v] = twice(0.f);
-  for (;;) {
-    const uint4 *xd = in.map(0), *gd = in.map(1);
-    const long long first = in.now.off + c0;
-    stage_rows<kVecs<2>>(at, in.now.rows, [&](int i, int row) {
-      float2 d[V / 2], g[V / 2];
-      Vec2<T>::unpack(xd[i], d);
-      Vec2<T>::unpack(gd[i], g);
-      f.apply(p, first + (long long)row * p.C, d, g);
-#pragma unroll
-      for (int v = 0; v < V / 2; ++v) {
-        sa[v] = add2(sa[v], g[v]);
-        sx[v] = fma2(g[v], d[v], sx[v]);
-      }
-    });
-    const bool last = in.now.flags & kLast;
-    in.close();
-    if (last) break;
-    if (!in.open()) return false;
-  }
-#pragma unroll
-  for (int v = 0; v < V / 2; ++v)
-    reinterpret_cast<float4*>(sums)[threadIdx.x * V / 2 + v] =
-        make_float4(sa[v].x, sx[v].x, sa[v].y, sx[v].y);
+// Adds up what the CTA's threads have in `sums` [rp, C], in float64: the parameters' gradients
+// into the CTA's own row of p.sums, the groups' sums into acc [G] (from 0 if `first`), and
+// with `last` the latter into the segment's entries. Every arithmetic thread calls it.
+template <typename T>
+__device__ __forceinline__ void reduce_sums(const NormArgs& p, const Place& at, int b, int seg,
+                                            float2* sums, double2* acc, bool first, bool last,
+                                            bool* started) {
   stream_sync();
-  // Channel sums in place, those of the parameters' gradients into the CTA's own row:
-  // X = r sum dz (x - mu), the sums centred on mu rounded to float32.
+  // X = r sum dz (x - mu), the sums centred on mu rounded to float32
   const double2* stats = p.stats + (long long)b * p.G;
   const bool params = p.dweight || p.dbias;
   for (int c = threadIdx.x; c < p.C; c += kS) {
-    float2 v = sums[c];
+    double2 v = as_double2(sums[c]);
     for (int r = 1; r < at.rp; ++r) {
       const float2 e = sums[r * p.C + c];
       v.x += e.x;
       v.y += e.y;
     }
-    sums[c] = v;
+    if (at.rp > 1) {  // the channel's sum in place, as float pairs
+      const float2 high = make_float2((float)v.x, (float)v.y);
+      sums[c] = high;
+      sums[p.C + c] = make_float2((float)(v.x - high.x), (float)(v.y - high.y));
+    }
     if (params) {
       const double2 st = __ldg(stats + c / p.Cg);
       double2* row = p.sums + (long long)blockIdx.x * p.C + c;
       double2 t = *started ? *row : make_double2(0.0, 0.0);
       t.x += v.x;
-      t.y += st.y * ((double)v.y - (st.x - (double)(float)st.x) * v.x);
+      t.y += st.y * (v.y - (st.x - (double)(float)st.x) * v.x);
       *row = t;
     }
   }
@@ -743,17 +721,78 @@ __device__ __forceinline__ bool grad_sums_unit(const NormArgs& p, const Place& a
         for (int i = lane; i < p.Cg; i += width) {
           const int c = g * p.Cg + i;
           const double w = param_f<T>(p.weight, p.param_f32, c, 1.f);
-          const float2 e = sums[c];
+          double2 e = as_double2(sums[c]);
+          if (at.rp > 1) {
+            const float2 low = sums[p.C + c];
+            e.x += low.x;
+            e.y += low.y;
+          }
           t.x += w * e.x;
           t.y += w * e.y;
         }
       }
       t = lanes_sum(t, width);
-      if (g < p.G && lane == 0) put(p.part + (long long)seg * p.G + g, entry_of(t));
+      if (g < p.G && lane == 0) {
+        if (!first) {
+          t.x += acc[g].x;
+          t.y += acc[g].y;
+        }
+        if (last) put(p.part + (long long)seg * p.G + g, entry_of(t));
+        else acc[g] = t;
+      }
     }
     stream_sync();  // the sums have been read
   }
-  return true;
+}
+
+template <typename T, bool WHOLE, bool RECT, bool DROP, typename C>
+__device__ __forceinline__ bool grad_sums_unit(const NormArgs& p, const Place& at, C& in,
+                                               float2* sums, double2* acc, bool* started) {
+  constexpr int V = 16 / sizeof(T), kFold = kRun / kVecs<2>;  // stages of a run
+  const int b = in.now.b, seg = in.now.seg, c0 = at.col * V;
+  Slope<T, WHOLE, RECT, DROP> f(p, b, c0);
+  float2 sa[V / 2], sx[V / 2];
+#pragma unroll
+  for (int v = 0; v < V / 2; ++v) sa[v] = sx[v] = twice(0.f);
+  float4* mine = reinterpret_cast<float4*>(sums) + threadIdx.x * (V / 2);
+  bool first = true;
+  for (int n = 1;; ++n) {
+    const uint4 *xd = in.map(0), *gd = in.map(1);
+    const long long from = in.now.off + c0;
+    stage_rows<kVecs<2>>(at, in.now.rows, [&](int i, int row) {
+      float2 d[V / 2], g[V / 2];
+      Vec2<T>::unpack(xd[i], d);
+      Vec2<T>::unpack(gd[i], g);
+      f.apply(p, from + (long long)row * p.C, d, g);
+#pragma unroll
+      for (int v = 0; v < V / 2; ++v) {
+        sa[v] = add2(sa[v], g[v]);
+        sx[v] = fma2(g[v], d[v], sx[v]);
+      }
+    });
+    const bool last = in.now.flags & kLast;
+    in.close();
+    if (last || n % kFold == 0) {
+      // a run of rows ends: its sums go to the thread's own in shared memory
+#pragma unroll
+      for (int v = 0; v < V / 2; ++v) {
+        float4 t = make_float4(sa[v].x, sx[v].x, sa[v].y, sx[v].y);
+        if (n > kFold) {
+          const float4 e = mine[v];
+          t = make_float4(t.x + e.x, t.y + e.y, t.z + e.z, t.w + e.w);
+        }
+        mine[v] = t;
+        sa[v] = sx[v] = twice(0.f);
+      }
+      if (last || n == kFold * kRuns) {
+        reduce_sums<T>(p, at, b, seg, sums, acc, first, last, started);
+        first = false;
+        n = 0;
+      }
+    }
+    if (last) return true;
+    if (!in.open()) return false;
+  }
 }
 
 template <typename T, bool WHOLE, bool RECT, bool DROP, typename C>
@@ -814,7 +853,9 @@ __global__ void __launch_bounds__(kBlock, kPerSm) norm_backward_stream(NormArgs 
     if (in.now.flags & kSecond
             ? !grad_input_unit<T, WHOLE, RECT, DROP>(p, at, in, reinterpret_cast<double2*>(sh.sums),
                                                             sh.coef)
-            : !grad_sums_unit<T, WHOLE, RECT, DROP>(p, at, in, sh.sums, &started))
+            : !grad_sums_unit<T, WHOLE, RECT, DROP>(p, at, in, sh.sums,
+                                                    reinterpret_cast<double2*>(sh.coef),
+                                                    &started))
       break;
   }
   if (!started && (p.dweight || p.dbias))

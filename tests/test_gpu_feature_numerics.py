@@ -108,6 +108,42 @@ def test_constant_groups_give_the_bias(shape, groups):
     assert torch.equal(lc.group_norm(x, groups, None, b), b.expand(shape))
 
 
+# one streamed sample with 1024 and 2100 rows a thread; streamed with many rows of threads and
+# several chunks; plain kernels, one to four bytes a thread; whole samples
+LONG = [((1, 296 * 1024, 1024), 8, torch.float32), ((1, 296 * 2100, 1024), 8, torch.float32),
+        ((6, 200_000, 64), 64, torch.float32),
+        ((1, 296 * 1100, 1000), 8, torch.bfloat16), ((1, 400_000, 33), 3, torch.float32),
+        ((2, 500_000, 1), 1, torch.float16), ((1, 8192, 1), 1, torch.float32)]
+
+
+@pytest.mark.parametrize("value", [1.1, 1.7, 1 / 303104])
+@pytest.mark.parametrize("shape,groups,dtype", LONG)
+def test_equal_gradients_of_many_rows(shape, groups, dtype, value):
+    # the gradient of a mean: equal terms, whose float32 sums all round the same way
+    x = _randn(shape, 4, torch.float32).to(dtype).requires_grad_(True)
+    b = torch.zeros(shape[-1], device=DEV, requires_grad=True)
+    dy = torch.full((), value, dtype=dtype, device=DEV).expand(shape).contiguous()
+    term = float(dy.view(-1)[0])
+    y = lc.group_norm(x, groups, None, b)
+    gx, gb = torch.autograd.grad(y, (x, b), dy)
+    # 32 equal terms: partial sums k t, k = 2 ... 32, rounded by 2^-24 of themselves, 16.5 2^-24
+    # of the sum; again for 32 such sums; a thread's, a slice's and the result's own rounding
+    e = (2 * 16.5 + 3) * 2.0 ** -24
+    want = term * (x.numel() // shape[-1])
+    assert float((gb.double() - want).abs().max()) <= e * want
+    # dx = r (dz - mean dz - xhat mean(dz xhat)) is 0 but for xhat's mean (and that of its
+    # square over n); dz, the mean's error and the products are 1 + e + 4 2^-24 of r dz
+    v = _by_group(x.detach(), groups)
+    var = v.var((1, 3), correction=0, keepdim=True)
+    r = 1 / (var + 1e-5).sqrt()
+    xhat = ((v - v.mean((1, 3), keepdim=True)) * r).abs()
+    # sum dz (x - mu): the terms are not equal; e of the sum of their magnitudes
+    m2 = e * xhat.mean((1, 3), keepdim=True)
+    tol = r * term * (e + 4 * 2.0 ** -24 + xhat * (m2 + 4 * 2.0 ** -24))
+    got = _by_group(gx, groups).abs()
+    assert bool((got <= tol * (1 + torch.finfo(dtype).eps)
+                 + torch.finfo(dtype).smallest_normal).all())
+
 # ---------------------------------------------------------------------------
 # what autograd is told
 # ---------------------------------------------------------------------------
