@@ -19,6 +19,7 @@ import contextlib
 import functools
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -118,6 +119,13 @@ def _check_residual(x, residual):
         raise ValueError(
             f"dropout: the residual must be like x, {x.dtype} {tuple(x.shape)} on {x.device}, "
             f"but got {residual.dtype} {tuple(residual.shape)} on {residual.device}")
+
+
+def _check_tangents(what, *tensors):
+    """Refuses forward-mode differentiation: a launch would drop the tangents without a word."""
+    if forward_ad._current_level >= 0 and any(
+            t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError(f"{what} has no forward-mode derivative (jvp)")
 
 
 def _check_used(used, p, grad, what):
@@ -342,6 +350,7 @@ def group_norm(x, num_groups, weight=None, bias=None, eps=1e-5, activation="none
               dropout_mode == "channel")
     if torch.compiler.is_compiling():
         return torch.ops.localcorr.group_norm(x, weight, bias, *params, tensor, seed, offset)[0]
+    _check_tangents("group_norm", x, weight, bias)
     if torch.is_grad_enabled() and (x.requires_grad
                                     or (weight is not None and weight.requires_grad)
                                     or (bias is not None and bias.requires_grad)):
@@ -361,7 +370,7 @@ def dropout(x, p, rng, residual=None, mode="element"):
     between replays. Equal (seed, offset) give equal masks, so every dropout of
     a step takes an offset of its own. No mask is stored: the backward
     pass draws it again from a copy of the stream that the forward kept. Call it
-    in training only (``p = 0`` copies x).
+    in training only (``p = 0`` copies x). Gradients as for :func:`group_norm`.
     """
     _check_map(x, "dropout")
     p = _check_dropout(p, rng, mode, x, "dropout")
@@ -370,6 +379,7 @@ def dropout(x, p, rng, residual=None, mode="element"):
     args = (x, residual, p, mode == "channel", tensor, seed, offset)
     if torch.compiler.is_compiling():
         return torch.ops.localcorr.dropout(*args)[0]
+    _check_tangents("dropout", x, residual)
     if torch.is_grad_enabled() and (x.requires_grad
                                     or (residual is not None and residual.requires_grad)):
         return DropoutFunction.apply(*args)

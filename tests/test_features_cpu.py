@@ -215,3 +215,13 @@ def test_only_the_map_of_a_registered_operator_is_differentiable():
         assert y.requires_grad and not stats.requires_grad and not used.requires_grad
         y, used = torch.ops.localcorr.dropout(x, x, 0.5, True, None, 1, 2)
         assert y.requires_grad and not used.requires_grad
+
+
+def test_tangents_are_refused():
+    x = torch.ones(2, 8)
+    features._check_tangents("dropout", x, None)
+    with torch.autograd.forward_ad.dual_level():
+        features._check_tangents("dropout", x, None)
+        dual = torch.autograd.forward_ad.make_dual(x, x)
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            features._check_tangents("dropout", x, dual)

@@ -161,3 +161,20 @@ def test_by_products_of_registered_operators_are_not_differentiable():
         stats.sum().backward()
     y, used = op.dropout(x, x, 0.5, True, None, 1, 2)
     assert y.requires_grad and not used.requires_grad
+
+
+def test_other_kinds_of_differentiation_are_refused():
+    x = _randn((2, 30, 16), 5).float()
+    w = torch.ones(16, device=DEV)
+    calls = (lambda t: lc.group_norm(t, 4), lambda t: lc.group_norm(x, 4, w, t[0, 0]),
+             lambda t: lc.dropout(t, 0.5, (1, 2)), lambda t: lc.dropout(x, 0.5, (1, 2), residual=t))
+    for call in calls:
+        with torch.autograd.forward_ad.dual_level():
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call(torch.autograd.forward_ad.make_dual(x, torch.ones_like(x)))
+        with pytest.raises(RuntimeError):
+            torch.func.jvp(call, (x,), (torch.ones_like(x),))
+        with pytest.raises(RuntimeError):
+            torch.func.vmap(call)(x.expand(3, 2, 30, 16))
+        with pytest.raises(RuntimeError):
+            torch.func.grad(lambda t: call(t).sum())(x)
