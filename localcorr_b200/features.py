@@ -290,8 +290,8 @@ class GroupNormFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, params, rng, seed, offset):
         x = x.contiguous()
-        y, ctx.stats, ctx.used = group_norm_forward(x, weight, bias, *params, rng, seed, offset)
-        ctx.save_for_backward(x, weight, bias)
+        y, stats, used = group_norm_forward(x, weight, bias, *params, rng, seed, offset)
+        ctx.save_for_backward(x, weight, bias, stats, used)
         ctx.params = params
         return y
 
@@ -300,8 +300,8 @@ class GroupNormFunction(torch.autograd.Function):
     def backward(ctx, grad_y):
         num_groups, _, activation, negative_slope, p, channel = ctx.params
         nx, nw, nb = ctx.needs_input_grad[:3]
-        return (*group_norm_backward(grad_y, *ctx.saved_tensors, ctx.stats, ctx.used, num_groups,
-                                     activation, negative_slope, p, channel, nx, nw, nb),
+        return (*group_norm_backward(grad_y, *ctx.saved_tensors, num_groups, activation,
+                                     negative_slope, p, channel, nx, nw, nb),
                 None, None, None, None)
 
 
@@ -310,14 +310,15 @@ class DropoutFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, residual, p, channel, rng, seed, offset):
-        y, ctx.used = dropout_forward(x, residual, p, channel, rng, seed, offset)
+        y, used = dropout_forward(x, residual, p, channel, rng, seed, offset)
+        ctx.save_for_backward(used)
         ctx.params = (p, channel)
         return y
 
     @staticmethod
     @_once_differentiable
     def backward(ctx, grad_y):
-        gx = (dropout_backward(grad_y, ctx.used, *ctx.params)
+        gx = (dropout_backward(grad_y, *ctx.saved_tensors, *ctx.params)
               if ctx.needs_input_grad[0] else None)
         gr = grad_y if ctx.needs_input_grad[1] else None
         return gx, gr, None, None, None, None, None

@@ -178,3 +178,31 @@ def test_other_kinds_of_differentiation_are_refused():
             torch.func.vmap(call)(x.expand(3, 2, 30, 16))
         with pytest.raises(RuntimeError):
             torch.func.grad(lambda t: call(t).sum())(x)
+
+
+def test_hooks_see_all_that_is_saved():
+    # what the backward needs lives where the graph's hooks (offloading) can move it
+    x = _randn((2, 30, 16), 6).float().requires_grad_(True)
+    w = torch.ones(16, device=DEV, requires_grad=True)
+    seen = []
+
+    def pack(t):
+        seen.append((tuple(t.shape), t.dtype))
+        return t.cpu()
+
+    for call, kept in (
+            (lambda: lc.group_norm(x, 4, w, activation="silu", p=0.5, rng=(1, 2)),
+             [((2, 30, 16), torch.float32), ((16,), torch.float32), ((2, 4, 2), torch.float64),
+              ((2,), torch.int64)]),
+            (lambda: lc.dropout(x, 0.5, (1, 2), residual=x), [((2,), torch.int64)])):
+        seen.clear()
+        with torch.autograd.graph.saved_tensors_hooks(pack, lambda t: t.to(DEV)):
+            y = call()
+        assert seen == kept
+        assert torch.equal(torch.autograd.grad(y.sum(), x)[0],
+                           torch.autograd.grad(call().sum(), x)[0])
+        # and is gone after the backward, unless it is asked to stay
+        y = call()
+        torch.autograd.grad(y.sum(), x)
+        with pytest.raises(RuntimeError, match="second time"):
+            torch.autograd.grad(y.sum(), x)
