@@ -250,10 +250,17 @@ LCB200_API bool launchLocalCorrB200SpatialBackward(
 /* Message of the last failed call on this thread ("" if none). */
 LCB200_API const char* localCorrB200GetLastError(void);
 
-/* Error status raised on the device by the tensor-core kernels (0 = none;
- * 1 = a pipeline wait timed out and the kernel stopped early). Synchronises
- * with the current device; reset clears it. */
+/* Error status raised on the current device by the tensor-core kernels and the
+ * group norm's (0 = none; 1 = a wait inside a kernel ran out and the kernel
+ * stopped early: the outputs of a call since the last reset are unfinished).
+ * No call checks it by itself. Synchronises with the device; reset clears it. */
 LCB200_API int localCorrB200DeviceStatus(int reset);
+
+/* Limit of the waits inside the group norm's kernels, in nanoseconds, for the
+ * calls that follow (all host threads); 2e9 until it is set. Returns the one
+ * before; a negative value only reads it. A limit that a call's waits reach
+ * ends that call early and sets the status above. */
+LCB200_API long long localCorrB200SetNormWaitLimit(long long nanoseconds);
 
 /* Library ABI version (major*10000 + minor*100 + patch). */
 LCB200_API int localCorrB200Version(void);

@@ -146,6 +146,7 @@ PROTOTYPES = {
     ),
     "localCorrB200GetLastError": (ctypes.c_char_p, []),
     "localCorrB200DeviceStatus": (_c_int, [_c_int]),
+    "localCorrB200SetNormWaitLimit": (_c_longlong, [_c_longlong]),
     "localCorrB200Version": (_c_int, []),
     "localCorrB200LaunchCount": (ctypes.c_longlong, [_c_int]),
     "localCorrB200SetDeterministic": (None, [_c_int]),

@@ -53,6 +53,7 @@ bool tc_bwd_eligible(int B, int H1, int W1, int H2, int W2, int C, int radius, i
                      int dilation, int dtype, std::string* why);
 int tc_device_status(bool reset);
 int feature_device_status(bool reset);
+long long feature_wait_limit(long long ns);
 bool layout_nchw_to_nhwc(const void*, void*, int, int, int, int, cudaStream_t);
 bool layout_nhwc_to_nchw(const void*, void*, int, int, int, int, cudaStream_t);
 bool layout_pyramid_build(const void*, void*, int, int, int, int, int, int, cudaStream_t);
@@ -979,7 +980,12 @@ bool launchLocalCorrB200GroupNormBackward(
 const char* localCorrB200GetLastError(void) { return g_last_error.c_str(); }
 
 int localCorrB200DeviceStatus(int reset) {
+  cudaDeviceSynchronize();  // copies from symbols do not wait for non-blocking streams
   return tc_device_status(reset != 0) | feature_device_status(reset != 0);
+}
+
+long long localCorrB200SetNormWaitLimit(long long nanoseconds) {
+  return feature_wait_limit(nanoseconds);
 }
 
 int localCorrB200Version(void) { return 100; }

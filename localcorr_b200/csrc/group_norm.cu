@@ -3,6 +3,8 @@
 // number of aligned 16-byte vectors, too wide, or of too many groups. The plain kernels
 // move 1 to 2.5 TB/s where the streamed ones move 3 to 4 (8 x 32400 x 99 float16
 // element by element: 92 us forward; x 96: 35 us).
+#include <atomic>
+
 #include "norm_common.cuh"
 
 namespace lcb200 {
@@ -13,6 +15,8 @@ int stream_ctas();  // resident CTAs
 int stream_stage_rows(int C, int dtype, bool backward);  // rows of a stage, at least 1
 
 namespace {
+
+std::atomic<long long> wait_limit{2000000000};  // ns
 
 // ---- forward, first pass: slice sums, and the sample's statistics -----------------
 template <typename T, int V>
@@ -338,7 +342,7 @@ __global__ void __launch_bounds__(kT, kOcc) norm_forward_kernel(NormArgs p) {
         publish(p.ready + b);
       return true;
     }
-    if (!wait_for(p.ready + b)) return false;
+    if (!wait_for(p, p.ready + b)) return false;
     apply_slice<T, V, DROP>(p, b, j);
     return true;
   });
@@ -360,7 +364,7 @@ __global__ void __launch_bounds__(kT, kOcc) norm_backward_kernel(NormArgs p) {
       }
       return true;
     }
-    if (!wait_for(p.ready + b)) return false;
+    if (!wait_for(p, p.ready + b)) return false;
     grad_input_slice<T, V, DROP>(p, b, j, p.coef + (long long)b * p.G);
     return true;
   });
@@ -624,6 +628,7 @@ bool feature_norm(const void* x, const void* dy, const void* weight, const void*
   p.act = act;
   p.slope = slope;
   p.eps = eps;
+  p.wait_ns = (uint64_t)wait_limit.load(std::memory_order_relaxed);
   p.slices = q.slices;
   p.slice_rows = q.slice_rows;
   p.fan = q.fan;
@@ -659,6 +664,10 @@ bool feature_norm(const void* x, const void* dy, const void* weight, const void*
   if (dtype == LCB200_F32) return launch_params<float>(p, p.ctas * p.teams, s);
   if (dtype == LCB200_F16) return launch_params<__half>(p, p.ctas * p.teams, s);
   return launch_params<__nv_bfloat16>(p, p.ctas * p.teams, s);
+}
+
+long long feature_wait_limit(long long ns) {
+  return ns < 0 ? wait_limit.load() : wait_limit.exchange(ns);
 }
 
 int feature_device_status(bool reset) {

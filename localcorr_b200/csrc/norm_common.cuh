@@ -34,6 +34,7 @@
 #pragma once
 
 #include "feature_common.cuh"
+#include "tc_ptx.cuh"
 
 namespace lcb200 {
 
@@ -42,7 +43,6 @@ constexpr int kOcc = 3;      // CTAs a multiprocessor holds
 constexpr int kUnroll = 4;   // rows a thread has in flight
 constexpr int kRun = 32;     // rows of a thread whose terms are added in float32
 constexpr int kRuns = 32;    // such sums added in float32
-constexpr long long kWaitLimit = 1 << 24;  // polls (100 ns and more each) before a wait gives up
 
 // 1: a wait ran out and a kernel of this translation unit stopped early
 static __device__ int norm_status;
@@ -62,6 +62,7 @@ struct NormArgs {
   int act;
   float slope;
   double eps;
+  uint64_t wait_ns;     // after which a wait gives up
   int slices;           // of a sample
   long long slice_rows;
   int fan, sets;        // slices of a set (see finish_slice), sets of a sample
@@ -369,14 +370,15 @@ static inline int read_norm_status(bool reset) {
   return v;
 }
 
-// False when the wait ran out: the CTA stops.
-static __device__ bool wait_for(const uint32_t* flag) {
+// False, for every thread of the CTA, when the wait ran out: the CTA stops.
+static __device__ bool wait_for(const NormArgs& p, const uint32_t* flag) {
   __shared__ int ok;
   if (threadIdx.x == 0) {
+    const uint64_t t0 = tc::globaltimer();
     uint32_t v = 0;
-    for (long long i = 0; i < kWaitLimit; ++i) {
+    for (;;) {
       asm volatile("ld.acquire.gpu.u32 %0, [%1];" : "=r"(v) : "l"(flag) : "memory");
-      if (v) break;
+      if (v || tc::globaltimer() - t0 >= p.wait_ns) break;
       __nanosleep(100);
     }
     if (!v) atomicExch(&norm_status, 1);

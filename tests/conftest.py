@@ -27,3 +27,17 @@ def _restore_backend():
     saved = backend._onnx_backend
     yield
     backend._onnx_backend = saved
+
+
+@pytest.fixture(autouse=True)
+def _feature_kernels_finish(request):
+    """No wait inside a kernel runs out in the GPU tests of the feature-map operators."""
+    if not request.path.name.startswith("test_gpu_feature"):
+        yield
+        return
+    from localcorr_b200 import _lib
+
+    lib = _lib.require_library()
+    lib.localCorrB200DeviceStatus(1)
+    yield
+    assert lib.localCorrB200DeviceStatus(1) == 0, "a wait inside a kernel ran out"

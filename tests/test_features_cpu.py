@@ -225,3 +225,11 @@ def test_tangents_are_refused():
         dual = torch.autograd.forward_ad.make_dual(x, x)
         with pytest.raises(RuntimeError, match="forward-mode"):
             features._check_tangents("dropout", x, dual)
+
+
+def test_c_wait_limit(lib):
+    before = lib.localCorrB200SetNormWaitLimit(-1)
+    assert before == 2_000_000_000
+    assert lib.localCorrB200SetNormWaitLimit(5) == before
+    assert lib.localCorrB200SetNormWaitLimit(before) == 5
+    assert lib.localCorrB200SetNormWaitLimit(-1) == before
