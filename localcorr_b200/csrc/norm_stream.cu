@@ -37,6 +37,19 @@ __device__ __forceinline__ void stream_sync() {
   asm volatile("bar.sync 1, %0;" ::"n"(kS) : "memory");
 }
 
+// A barrier that tells every thread whether all of them came with true.
+__device__ __forceinline__ bool all_threads(bool ok) {
+  int r;
+  __syncwarp();
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.s32 q, %1, 0;\n\tbar.red.and.pred p, 1, %2, q;\n\t"
+      "selp.s32 %0, 1, 0, p;\n\t}"
+      : "=r"(r)
+      : "r"((int)ok), "n"(kS)
+      : "memory");
+  return r != 0;
+}
+
 __device__ __forceinline__ uint64_t bits(float2 v) { return *reinterpret_cast<uint64_t*>(&v); }
 __device__ __forceinline__ float2 pair(uint64_t v) { return *reinterpret_cast<float2*>(&v); }
 __device__ __forceinline__ float2 twice(float v) { return make_float2(v, v); }
@@ -151,18 +164,25 @@ __device__ __forceinline__ void put(void* p, const Entry& e) {
 // ---- the ring ------------------------------------------------------------------------
 struct StageInfo {
   long long off;  // element offset of the stage's first row
-  int rows;       // of the stage
   int b;          // sample
   int seg;        // slot of the segment's sums
-  int flags;
+  int rows;       // of the stage, and flags
 };
-enum : int { kSecond = 1, kLast = 2, kEnd = 4, kTop = 8 };  // kTop: starts the sample
+enum : int {
+  kRowsMask = 0xffff,
+  kSecond = 1 << 16,
+  kLast = 2 << 16,
+  kEnd = 4 << 16,
+  kTop = 8 << 16,  // starts the sample
+};
 
 template <int NM, int STAGES>
 struct RingShared {
   uint4 data[STAGES][NM][kVecs<NM> * kS];
   uint64_t full[STAGES], empty[STAGES];
   StageInfo info[STAGES];
+  int b, seg;   // of a first pass's unit, for its end
+  int started;  // whether the CTA's row of parameter sums holds something
   int abort;
 };
 
@@ -182,7 +202,7 @@ __device__ void ring_init(RingShared<NM, STAGES>& r) {
       tc::mbar_init(&r.full[i], 1);
       tc::mbar_init(&r.empty[i], kS / 32);
     }
-    r.abort = 0;
+    r.abort = r.started = 0;
     tc::fence_mbar_init();
   }
   __syncthreads();
@@ -234,7 +254,7 @@ __device__ void produce(const NormArgs& p, RingShared<NM, STAGES>& r, const T* m
   uint32_t n = 0;  // stages issued
   bool good = true;
   auto claim = [&]() {
-    return tc::mbar_wait(&r.empty[n % STAGES], ((n / STAGES) & 1) ^ 1, &r.abort);
+    return tc::mbar_wait(&r.empty[n % STAGES], ((n / STAGES) & 1) ^ 1, &r.abort, p.wait_ns);
   };
   auto run = [&](const Chunk& c, int q, bool second) {
     if (q >= c.parts) return;
@@ -251,7 +271,7 @@ __device__ void produce(const NormArgs& p, RingShared<NM, STAGES>& r, const T* m
         const uint32_t bytes = (uint32_t)(rows * p.C * sizeof(T));
         const long long off = ((long long)(c.first + s) * p.S + row) * p.C;
         r.info[at] =
-            StageInfo{off, rows, c.first + s, seg, flags | (t == stages - 1 ? kLast : 0)};
+            StageInfo{off, c.first + s, seg, rows | flags | (t == stages - 1 ? kLast : 0)};
         tc::mbar_arrive_expect_tx(&r.full[at], bytes * NM);
         bulk_copy(r.data[at][0], m0 + off, bytes, &r.full[at], policy);
         if (NM > 1) bulk_copy(r.data[at][NM - 1], m1 + off, bytes, &r.full[at], policy);
@@ -266,7 +286,7 @@ __device__ void produce(const NormArgs& p, RingShared<NM, STAGES>& r, const T* m
     if (p.out) run(c, q, true);
   }
   if (good && claim()) {
-    r.info[n % STAGES].flags = kEnd;
+    r.info[n % STAGES] = StageInfo{0, 0, 0, kEnd};
     tc::mbar_arrive(&r.full[n % STAGES]);
   } else {  // gave up: no copy may be in flight when the CTA ends
     for (uint32_t k = n > STAGES ? n - STAGES : 0; k < n; ++k)
@@ -274,30 +294,60 @@ __device__ void produce(const NormArgs& p, RingShared<NM, STAGES>& r, const T* m
   }
 }
 
-// The arithmetic warps' side.
+// The arithmetic warps' side. A wait that runs out (here or in poll) ends the kernel, but
+// threads see it at different times: one may give up on a copy that lands for another. So a
+// thread that gave up has a stage of no rows, its warp learns of it at the stage's end, and
+// the CTA at the next barrier that the unit has for all threads anyway (all_threads). No
+// thread leaves by itself, and none waits at a barrier for one that left. (The vote costs 1 %
+// of a backward pass: 8 x 540 x 960 x 64 float16 431 us with it and 427 without.)
 template <int NM, int STAGES>
 struct Consumer {
+  const NormArgs& p;
   RingShared<NM, STAGES>& r;
   uint32_t n = 0;
-  StageInfo now{};
+  long long off = 0;  // of the stage, see StageInfo
+  int now = 0;
 
-  __device__ __forceinline__ explicit Consumer(RingShared<NM, STAGES>& ring) : r(ring) {}
-  // Waits for the next stage; false at the end or when a wait ran out.
-  __device__ __forceinline__ bool open() {
-    if (!tc::mbar_wait(&r.full[n % STAGES], (n / STAGES) & 1, &r.abort)) {
+  __device__ __forceinline__ Consumer(const NormArgs& args, RingShared<NM, STAGES>& ring)
+      : p(args), r(ring) {}
+  // Waits for the next stage. now is 0 in a thread whose wait ran out.
+  __device__ __forceinline__ void open() {
+    if (tc::mbar_wait(&r.full[n % STAGES], (n / STAGES) & 1, &r.abort, p.wait_ns)) {
+      off = r.info[n % STAGES].off;
+      now = r.info[n % STAGES].rows;
+    } else {
       atomicExch(&norm_status, 1);
-      return false;
+      now = 0;
     }
-    now = r.info[n % STAGES];
-    return !(now.flags & kEnd);
   }
+  __device__ __forceinline__ int rows() const { return now & kRowsMask; }
+  __device__ __forceinline__ int sample() const { return r.info[n % STAGES].b; }
+  __device__ __forceinline__ int segment() const { return r.info[n % STAGES].seg; }
   __device__ __forceinline__ const uint4* map(int m) const { return r.data[n % STAGES][m]; }
-  __device__ __forceinline__ void close() {
-    __syncwarp();
-    if (threadIdx.x % 32 == 0) tc::mbar_arrive(&r.empty[n % STAGES]);
+  // The warp is done with the stage; false when it did not open for all of its threads: the
+  // stage then stays the producer's, whose copy may still be under way.
+  __device__ __forceinline__ bool close() {
+    const bool opened = __all_sync(0xffffffffu, now);
+    if (opened && threadIdx.x % 32 == 0) tc::mbar_arrive(&r.empty[n % STAGES]);
     ++n;
+    return opened;
   }
 };
+
+// Calls unit() for each unit's first stage until the producer's end, or until a wait ran out
+// for any thread. The barrier between units also keeps one unit's shared values until every
+// thread has read them.
+template <typename C, typename F>
+__device__ __forceinline__ void each_unit(C& in, F unit) {
+  bool ok = true;
+  for (;;) {
+    if (ok) in.open();
+    if (!all_threads(ok && in.now)) break;
+    if (in.now & kEnd) return;
+    ok = unit();
+  }
+  in.r.abort = 1;  // the producer stops too
+}
 
 // Calls row(i-th vector of the stage's map 0, row) for this thread's rows of a stage.
 template <int VECS, typename F>
@@ -316,17 +366,18 @@ __device__ __forceinline__ void stage_rows(const Place& at, int rows, F row) {
 }
 
 // ---- the sums of a sample ------------------------------------------------------------
-// Polls an entry that was not ready; gives up after two seconds, or when another
-// thread of the CTA did.
-__device__ __forceinline__ Entry poll(const void* p, volatile int* abort) {
+// Polls an entry that was not ready. Gives up when the limit is reached, or when another
+// thread of the CTA did, with NaN: the kernel ends at its next wait, and what it still
+// writes shows.
+__device__ __forceinline__ Entry poll(const void* p, uint64_t limit, volatile int* abort) {
   const uint64_t t0 = tc::globaltimer();
   for (uint32_t i = 1;; ++i) {
     const Entry e = get(p);
     if (e.ready()) return e;
-    if (i % 32 == 0 && (*abort || tc::globaltimer() - t0 > 2000000000ull)) {
+    if ((i % 32 == 0 || limit == 0) && (*abort || tc::globaltimer() - t0 >= limit)) {
       *abort = 1;
       atomicExch(&norm_status, 1);
-      return Entry{0, 0};
+      return Entry{0x7ff8000000000000ull, 0x7ff8000000000000ull};
     }
     __nanosleep(200);
   }
@@ -357,7 +408,8 @@ __device__ __forceinline__ void sample_sums(const NormArgs& p, int b, volatile i
         e[u] = get(part + (long long)min(at + u * 32, runs - 1) * p.G);
 #pragma unroll
       for (int u = 0; u < kFlight; ++u)
-        if (!e[u].ready()) poll(part + (long long)min(at + u * 32, runs - 1) * p.G, abort);
+        if (!e[u].ready())
+          poll(part + (long long)min(at + u * 32, runs - 1) * p.G, p.wait_ns, abort);
     }
   }
   stream_sync();
@@ -380,7 +432,8 @@ __device__ __forceinline__ void sample_sums(const NormArgs& p, int b, volatile i
 #pragma unroll
         for (int u = 0; u < kFlight; ++u) {
           if (at + u * step < runs) {
-            if (!e[u].ready()) e[u] = poll(src + (long long)(at + u * step) * p.G, abort);
+            if (!e[u].ready())
+              e[u] = poll(src + (long long)(at + u * step) * p.G, p.wait_ns, abort);
             const double2 d = pair_of(e[u]);
             v.x += d.x;
             v.y += d.y;
@@ -424,11 +477,12 @@ __device__ __forceinline__ bool stats_unit(const NormArgs& p, const Place& at, C
 #pragma unroll
   for (int v = 0; v < A; ++v) s[v] = q[v] = 0.0;
 #pragma unroll
-  for (int v = 0; v < N; ++v) k[v] = group_shift<T>(p, in.now.b, (at.col * V + v) / p.Cg);
-  const int seg = in.now.seg;
+  for (int v = 0; v < N; ++v) k[v] = group_shift<T>(p, in.sample(), (at.col * V + v) / p.Cg);
+  const int seg = in.segment();
+  bool ok = true;
   for (;;) {
     const uint4* data = in.map(0);
-    stage_rows<kVecs<1>>(at, in.now.rows, [&](int i, int) {
+    stage_rows<kVecs<1>>(at, in.rows(), [&](int i, int) {
       float2 f[V / 2];
       Vec2<T>::unpack(data[i], f);
 #pragma unroll
@@ -438,10 +492,10 @@ __device__ __forceinline__ bool stats_unit(const NormArgs& p, const Place& at, C
         q[v % A] = fma(d, d, q[v % A]);
       }
     });
-    const bool last = in.now.flags & kLast;
-    in.close();
-    if (last) break;
-    if (!in.open()) return false;
+    const bool last = in.now & kLast;
+    ok = in.close();
+    if (last || !ok) break;
+    in.open();
   }
   if (WHOLE) {
     sh.sums[threadIdx.x] = make_double2(s[0] + s[1], q[0] + q[1]);
@@ -449,7 +503,7 @@ __device__ __forceinline__ bool stats_unit(const NormArgs& p, const Place& at, C
 #pragma unroll
     for (int v = 0; v < N; ++v) sh.sums[threadIdx.x * N + v] = make_double2(s[v], q[v]);
   }
-  stream_sync();
+  if (!all_threads(ok)) return false;
   // one group by `width` lanes
   const int ne = at.nc * N, gw = p.Cg * N / V;
   const int width = min(32, max(1, pow2_below(min(at.rp * gw, kS / min(p.G, kS)))));
@@ -468,7 +522,6 @@ __device__ __forceinline__ bool stats_unit(const NormArgs& p, const Place& at, C
     t = lanes_sum(t, width);
     if (g < p.G && lane == 0) put(p.part + (long long)seg * p.G + g, entry_of(t));
   }
-  stream_sync();  // the sums have been read
   return true;
 }
 
@@ -476,9 +529,8 @@ template <typename T, bool WHOLE, bool DROP, typename C>
 __device__ __forceinline__ bool apply_unit(const NormArgs& p, const Place& at, C& in,
                                            double2* red, double2* stats) {
   constexpr int V = 16 / sizeof(T), N = WHOLE ? 1 : V / 2;
-  const int b = in.now.b, c0 = at.col * V;
-  const bool top = in.now.flags & kTop;
-  stream_sync();  // the last sample's have been read
+  const int b = in.sample(), c0 = at.col * V;
+  const bool top = in.now & kTop;
   // on their way while the sums are: sample_sums starts with a barrier
   for (int g = threadIdx.x; g < p.G; g += kS) stats[g].x = group_shift<T>(p, b, g);
   sample_sums(p, b, &in.r.abort, red, [&](int g, double2 t) {
@@ -514,8 +566,8 @@ __device__ __forceinline__ bool apply_unit(const NormArgs& p, const Place& at, C
   const int act = p.act;
   for (;;) {
     const uint4* data = in.map(0);
-    const long long first = in.now.off + c0;
-    stage_rows<kVecs<1>>(at, in.now.rows, [&](int i, int row) {
+    const long long first = in.off + c0;
+    stage_rows<kVecs<1>>(at, in.rows(), [&](int i, int row) {
       float2 x[V / 2];
       Vec2<T>::unpack(data[i], x);
       const long long e = first + (long long)row * p.C;
@@ -551,10 +603,10 @@ __device__ __forceinline__ bool apply_unit(const NormArgs& p, const Place& at, C
       }
       __stcs(reinterpret_cast<uint4*>(dst + e), r);
     });
-    const bool last = in.now.flags & kLast;
-    in.close();
+    const bool last = in.now & kLast;
+    if (!in.close()) return false;
     if (last) return true;
-    if (!in.open()) return false;
+    in.open();
   }
 }
 
@@ -572,13 +624,11 @@ __global__ void __launch_bounds__(kBlock, kPerSm) norm_forward_stream(NormArgs p
     return;
   }
   const Place at(p.C / (16 / (int)sizeof(T)), 0, kS);
-  Consumer<1, ForwardShared<T, WHOLE>::kStages> in(sh.ring);
-  while (in.open()) {
-    if (in.now.flags & kSecond ? !apply_unit<T, WHOLE, DROP>(p, at, in, sh.sums, sh.stats)
-                               : !stats_unit<T, WHOLE>(p, at, in, sh))
-      break;
-  }
-  if (!(in.now.flags & kEnd)) sh.ring.abort = 1;
+  Consumer<1, ForwardShared<T, WHOLE>::kStages> in(p, sh.ring);
+  each_unit(in, [&]() {
+    return in.now & kSecond ? apply_unit<T, WHOLE, DROP>(p, at, in, sh.sums, sh.stats)
+                                  : stats_unit<T, WHOLE>(p, at, in, sh);
+  });
 }
 
 // ---- backward ------------------------------------------------------------------------
@@ -679,12 +729,15 @@ struct Slope {
 
 // Adds up what the CTA's threads have in `sums` [rp, C], in float64: the parameters' gradients
 // into the CTA's own row of p.sums, the groups' sums into acc [G] (from 0 if `first`), and
-// with `last` the latter into the segment's entries. Every arithmetic thread calls it.
-template <typename T>
-__device__ __forceinline__ void reduce_sums(const NormArgs& p, const Place& at, int b, int seg,
-                                            float2* sums, double2* acc, bool first, bool last,
-                                            bool* started) {
-  stream_sync();
+// with `last` the latter into the segment's entries. Every arithmetic thread calls it; false
+// when one of them comes without its sums.
+template <typename T, typename R>
+__device__ __forceinline__ bool reduce_sums(const NormArgs& p, const Place& at, R& ring,
+                                            float2* sums, double2* acc, bool ok, bool first,
+                                            bool last) {
+  if (!all_threads(ok)) return false;
+  const int b = ring.b, seg = ring.seg;
+  const bool started = ring.started;
   // X = r sum dz (x - mu), the sums centred on mu rounded to float32
   const double2* stats = p.stats + (long long)b * p.G;
   const bool params = p.dweight || p.dbias;
@@ -703,14 +756,14 @@ __device__ __forceinline__ void reduce_sums(const NormArgs& p, const Place& at, 
     if (params) {
       const double2 st = __ldg(stats + c / p.Cg);
       double2* row = p.sums + (long long)blockIdx.x * p.C + c;
-      double2 t = *started ? *row : make_double2(0.0, 0.0);
+      double2 t = started ? *row : make_double2(0.0, 0.0);
       t.x += v.x;
       t.y += st.y * (v.y - (st.x - (double)(float)st.x) * v.x);
       *row = t;
     }
   }
-  *started = true;
   stream_sync();
+  if (threadIdx.x == 0) ring.started = 1;
   if (p.out) {
     const int width = min(32, max(1, pow2_below(min(p.Cg, kS / min(p.G, kS)))));
     const int lane = threadIdx.x % width;
@@ -741,25 +794,30 @@ __device__ __forceinline__ void reduce_sums(const NormArgs& p, const Place& at, 
         else acc[g] = t;
       }
     }
-    stream_sync();  // the sums have been read
+    if (!last) stream_sync();  // the sums have been read
   }
+  return true;
 }
 
 template <typename T, bool WHOLE, bool RECT, bool DROP, typename C>
 __device__ __forceinline__ bool grad_sums_unit(const NormArgs& p, const Place& at, C& in,
-                                               float2* sums, double2* acc, bool* started) {
+                                               float2* sums, double2* acc) {
   constexpr int V = 16 / sizeof(T), kFold = kRun / kVecs<2>;  // stages of a run
-  const int b = in.now.b, seg = in.now.seg, c0 = at.col * V;
-  Slope<T, WHOLE, RECT, DROP> f(p, b, c0);
+  const int c0 = at.col * V;
+  Slope<T, WHOLE, RECT, DROP> f(p, in.sample(), c0);
+  if (threadIdx.x == 0) {
+    in.r.b = in.sample();
+    in.r.seg = in.segment();
+  }
   float2 sa[V / 2], sx[V / 2];
 #pragma unroll
   for (int v = 0; v < V / 2; ++v) sa[v] = sx[v] = twice(0.f);
   float4* mine = reinterpret_cast<float4*>(sums) + threadIdx.x * (V / 2);
-  bool first = true;
-  for (int n = 1;; ++n) {
+  constexpr int kAll = kFold * kRuns;  // stages until float64 takes over
+  for (int n = 0;;) {  // stages so far
     const uint4 *xd = in.map(0), *gd = in.map(1);
-    const long long from = in.now.off + c0;
-    stage_rows<kVecs<2>>(at, in.now.rows, [&](int i, int row) {
+    const long long from = in.off + c0;
+    stage_rows<kVecs<2>>(at, in.rows(), [&](int i, int row) {
       float2 d[V / 2], g[V / 2];
       Vec2<T>::unpack(xd[i], d);
       Vec2<T>::unpack(gd[i], g);
@@ -770,28 +828,28 @@ __device__ __forceinline__ bool grad_sums_unit(const NormArgs& p, const Place& a
         sx[v] = fma2(g[v], d[v], sx[v]);
       }
     });
-    const bool last = in.now.flags & kLast;
-    in.close();
-    if (last || n % kFold == 0) {
+    const bool last = in.now & kLast;
+    const bool ok = in.close();
+    const int at_run = n % kAll;  // of the stage in its runs
+    ++n;
+    if (last || !ok || n % kFold == 0) {
       // a run of rows ends: its sums go to the thread's own in shared memory
 #pragma unroll
       for (int v = 0; v < V / 2; ++v) {
         float4 t = make_float4(sa[v].x, sx[v].x, sa[v].y, sx[v].y);
-        if (n > kFold) {
+        if (at_run >= kFold) {
           const float4 e = mine[v];
           t = make_float4(t.x + e.x, t.y + e.y, t.z + e.z, t.w + e.w);
         }
         mine[v] = t;
         sa[v] = sx[v] = twice(0.f);
       }
-      if (last || n == kFold * kRuns) {
-        reduce_sums<T>(p, at, b, seg, sums, acc, first, last, started);
-        first = false;
-        n = 0;
+      if (last || !ok || n % kAll == 0) {
+        if (!reduce_sums<T>(p, at, in.r, sums, acc, ok, n <= kAll, last)) return false;
+        if (last) return true;
       }
     }
-    if (last) return true;
-    if (!in.open()) return false;
+    in.open();
   }
 }
 
@@ -799,8 +857,7 @@ template <typename T, bool WHOLE, bool RECT, bool DROP, typename C>
 __device__ __forceinline__ bool grad_input_unit(const NormArgs& p, const Place& at, C& in,
                                                 double2* red, float4* coef) {
   constexpr int V = 16 / sizeof(T), N = WHOLE ? 1 : V / 2;
-  const int b = in.now.b, c0 = at.col * V;
-  stream_sync();  // the last sample's have been read
+  const int b = in.sample(), c0 = at.col * V;
   sample_sums(p, b, &in.r.abort, red, [&](int g, double2 t) {
     coef[g] = finish_coef(p, __ldg(p.stats + (long long)b * p.G + g), t);
   });
@@ -816,8 +873,8 @@ __device__ __forceinline__ bool grad_input_unit(const NormArgs& p, const Place& 
   T* dst = reinterpret_cast<T*>(p.out);
   for (;;) {
     const uint4 *xd = in.map(0), *gd = in.map(1);
-    const long long first = in.now.off + c0;
-    stage_rows<kVecs<2>>(at, in.now.rows, [&](int i, int row) {
+    const long long first = in.off + c0;
+    stage_rows<kVecs<2>>(at, in.rows(), [&](int i, int row) {
       float2 d[V / 2], g[V / 2];
       Vec2<T>::unpack(xd[i], d);
       Vec2<T>::unpack(gd[i], g);
@@ -828,10 +885,10 @@ __device__ __forceinline__ bool grad_input_unit(const NormArgs& p, const Place& 
         g[v] = fma2(f.a[v], g[v], fma2(k2[WHOLE ? 0 : v % N], d[v], k3[WHOLE ? 0 : v % N]));
       __stcs(reinterpret_cast<uint4*>(dst + e), Vec2<T>::pack(g));
     });
-    const bool last = in.now.flags & kLast;
-    in.close();
+    const bool last = in.now & kLast;
+    if (!in.close()) return false;
     if (last) return true;
-    if (!in.open()) return false;
+    in.open();
   }
 }
 
@@ -847,21 +904,17 @@ __global__ void __launch_bounds__(kBlock, kPerSm) norm_backward_stream(NormArgs 
     return;
   }
   const Place at(p.C / (16 / (int)sizeof(T)), 0, kS);
-  Consumer<2, BackwardShared<T, WHOLE>::kStages> in(sh.ring);
-  bool started = false;  // whether this CTA's row of parameter sums holds something
-  while (in.open()) {
-    if (in.now.flags & kSecond
-            ? !grad_input_unit<T, WHOLE, RECT, DROP>(p, at, in, reinterpret_cast<double2*>(sh.sums),
-                                                            sh.coef)
-            : !grad_sums_unit<T, WHOLE, RECT, DROP>(p, at, in, sh.sums,
-                                                    reinterpret_cast<double2*>(sh.coef),
-                                                    &started))
-      break;
-  }
-  if (!started && (p.dweight || p.dbias))
+  Consumer<2, BackwardShared<T, WHOLE>::kStages> in(p, sh.ring);
+  each_unit(in, [&]() {
+    return in.now & kSecond
+               ? grad_input_unit<T, WHOLE, RECT, DROP>(p, at, in,
+                                                       reinterpret_cast<double2*>(sh.sums), sh.coef)
+               : grad_sums_unit<T, WHOLE, RECT, DROP>(p, at, in, sh.sums,
+                                                      reinterpret_cast<double2*>(sh.coef));
+  });
+  if (!sh.ring.started && (p.dweight || p.dbias))
     for (int c = threadIdx.x; c < p.C; c += kS)
       p.sums[(long long)blockIdx.x * p.C + c] = make_double2(0.0, 0.0);
-  if (!(in.now.flags & kEnd)) sh.ring.abort = 1;
 }
 
 // ---- host ----------------------------------------------------------------------------

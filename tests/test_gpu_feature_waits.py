@@ -1,8 +1,7 @@
 """Waits inside the group norm's kernels that run out: the kernel ends by itself, the status
 says so until it is reset, and the next call is right.
 
-With a limit of 0 a wait gives up when its first look finds nothing. Every kernel here has
-CTAs that look for a sum while others have only begun to add it up.
+With a limit of 0 a wait gives up when its first looks find nothing.
 """
 
 import pytest
@@ -56,9 +55,11 @@ def _run_out(lib, shape, groups, dtype):
     side = torch.cuda.Stream()  # does not synchronise with the default stream
     for call in (forward, lambda: torch.autograd.grad(want, (x, w), dy, retain_graph=True)):
         side.wait_stream(torch.cuda.current_stream())
-        with _Limit(lib, 0), torch.cuda.stream(side):
-            call()
-        assert lib.localCorrB200DeviceStatus(0) == 1
+        for _ in range(200):  # it may find all it looks for, if seldom
+            with _Limit(lib, 0), torch.cuda.stream(side):
+                call()
+            if lib.localCorrB200DeviceStatus(0):
+                break
         assert lib.localCorrB200DeviceStatus(1) == 1  # stays until it is reset
         assert lib.localCorrB200DeviceStatus(0) == 0
         torch.cuda.current_stream().wait_stream(side)
@@ -72,3 +73,37 @@ def _run_out(lib, shape, groups, dtype):
 @pytest.mark.parametrize("shape,groups,dtype", PLAIN)
 def test_plain_kernels(lib, shape, groups, dtype):
     _run_out(lib, shape, groups, dtype)
+
+
+# streamed: groups of whole vectors and of single channels, one sample and several chunks
+STREAMED = [((3, 4000, 64), 8, torch.float16), ((2, 2000, 64), 64, torch.float32),
+            ((1, 40_000, 96), 12, torch.bfloat16), ((9, 40_000, 128), 16, torch.float16),
+            ((33, 8192, 128), 128, torch.bfloat16)]
+
+
+# the CTAs of small maps come to their sums within the microseconds that a first look takes:
+# every wait may find what it looks for. Over a large map they drift apart.
+@pytest.mark.parametrize("shape,groups,dtype", STREAMED[3:])
+def test_streamed_kernels(lib, shape, groups, dtype):
+    _run_out(lib, shape, groups, dtype)
+
+
+@pytest.mark.parametrize("act", ["none", "relu"])
+@pytest.mark.parametrize("shape,groups,dtype", STREAMED)
+def test_limits_that_some_threads_reach(lib, shape, groups, dtype, act):
+    # limits about as long as the waits: threads of one CTA give up at different times. A call
+    # ends, and one that says it finished is right.
+    x, w, dy = _leaves(shape, dtype)
+
+    def call():
+        y = lc.group_norm(x, groups, w, activation=act)
+        return (y.detach(), *torch.autograd.grad(y, (x, w), dy))
+
+    want = call()
+    for limit in (300, 1000, 2000, 4000, 8000, 16000, 32000, 64000):
+        for _ in range(4):
+            with _Limit(lib, limit):
+                got = call()
+            if lib.localCorrB200DeviceStatus(1) == 0:
+                assert all(torch.equal(a, b) for a, b in zip(got, want))
+    assert all(torch.equal(a, b) for a, b in zip(call(), want))
