@@ -302,8 +302,8 @@ LCB200_API bool launchLocalCorrB200PyramidBackwardFmap2Pull(
 /* ---- Feature-map operators ---------------------------------------------------
  * No reference counterpart (the reference leaves the encoder to torch). The
  * maps are channels last, [B, rows, C] contiguous, rows the product of the
- * spatial sizes; dtype float32, float16 or bfloat16. Results are rounded to
- * dtype once. No float atomics: equal inputs give equal bits.
+ * spatial sizes, C at most 2^30; dtype float32, float16 or bfloat16. Results
+ * are rounded to dtype once. No float atomics: equal inputs give equal bits.
  *
  * Dropout draws: Philox4x32-10 with key seed and counter (block, offset);
  * draw e is 16-bit piece e % 8 (low half of a word first) of block e / 8, and

@@ -543,6 +543,10 @@ bool validate_feature(int B, long long rows, int C, int dtype, bool* empty) {
               ", C=" + std::to_string(C));
     return false;
   }
+  if (C > 1 << 30) {  // column loops step past the last one in 32 bits
+    set_error("at most 2^30 channels, got " + std::to_string(C));
+    return false;
+  }
   if ((double)B * (double)rows * (double)C > 1e18) {
     set_error("too many elements");
     return false;

@@ -233,3 +233,12 @@ def test_c_wait_limit(lib):
     assert lib.localCorrB200SetNormWaitLimit(5) == before
     assert lib.localCorrB200SetNormWaitLimit(before) == 5
     assert lib.localCorrB200SetNormWaitLimit(-1) == before
+
+
+def test_c_refuses_more_channels_than_the_kernels_count(lib):
+    # their column loops add up to 256 to a 32-bit column before they compare it
+    for c in (2 ** 30 + 1, 2 ** 31 - 1):
+        assert not _dropout(lib, c=c) and "channels" in _lib.last_error(lib)
+        assert not _forward(lib, c=c, g=1) and "channels" in _lib.last_error(lib)
+        assert lib.localCorrB200GroupNormWorkspaceBytes(1, 1, c, 1, _lib.F16, False) == 0
+    assert not _forward(lib, c=2 ** 30, g=1) and "workspace" in _lib.last_error(lib)
