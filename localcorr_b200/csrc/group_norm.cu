@@ -26,7 +26,7 @@ __device__ void stats_slice(const NormArgs& p, int b, int j, double2* out, doubl
   const T* xb = reinterpret_cast<const T*>(p.x) + (long long)b * p.S * p.C;
   const bool whole = p.Cg % V == 0;  // a vector lies in one group
   const int per = whole ? 1 : V;     // shared entries of a thread
-  const int gw = p.Cg * per / V;     // entries of one group and row (whole: Cg / V)
+  const int gw = whole ? p.Cg / V : p.Cg;  // entries of one group and row
   for (int cb = 0; cb < cols; cb += kT) {
     const Place at(cols, cb);
     if (at.on) {

@@ -108,6 +108,26 @@ def test_constant_groups_give_the_bias(shape, groups):
     assert torch.equal(lc.group_norm(x, groups, None, b), b.expand(shape))
 
 
+def test_groups_whose_vectors_pass_32_bits():
+    # 268435460 channels a group, no whole number of vectors: eight times that passes 2^31
+    c = 2 * 268_435_460
+    x = torch.empty(1, c, dtype=torch.float16, device=DEV).normal_(
+        generator=torch.Generator(DEV).manual_seed(7))
+    x[0, c // 2:] += 2.0
+    got_mean, got_rstd = _kernel_statistics(x, 2, 1e-5)
+    want_mean, want_rstd = _statistics(x, 2, 1e-5)
+    # 2^20 sequential float64 sums of a thread, 6 spreads from the group's first value at most
+    torch.testing.assert_close(got_mean, want_mean, rtol=0, atol=2.0 ** -28)
+    torch.testing.assert_close(got_rstd, want_rstd, rtol=2.0 ** -28, atol=0)
+    y = lc.group_norm(x, 2)
+    for lo in (0, c // 2 - 2048, c // 2, c - 2048):  # both ends of both groups
+        g = lo // (c // 2)
+        part = slice(lo, lo + 2048)
+        want = (x[0, part].double() - want_mean[0, g]) * want_rstd[0, g]
+        assert bool(((y[0, part].double() - want).abs()
+                     <= 2.0 ** -11 * want.abs() + 2.0 ** -20).all())
+
+
 # one streamed sample with 1024 and 2100 rows a thread; streamed with many rows of threads and
 # several chunks; plain kernels, one to four bytes a thread; whole samples
 LONG = [((1, 296 * 1024, 1024), 8, torch.float32), ((1, 296 * 2100, 1024), 8, torch.float32),
