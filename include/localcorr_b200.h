@@ -256,10 +256,11 @@ LCB200_API const char* localCorrB200GetLastError(void);
  * No call checks it by itself. Synchronises with the device; reset clears it. */
 LCB200_API int localCorrB200DeviceStatus(int reset);
 
-/* Limit of the waits inside the group norm's kernels, in nanoseconds, for the
- * calls that follow (all host threads); 2e9 until it is set. Returns the one
- * before; a negative value only reads it. A limit that a call's waits reach
- * ends that call early and sets the status above. */
+/* Limit of the waits inside the group norm's kernels, in nanoseconds for each
+ * started GB of the map, for the calls that follow (all host threads); 2e9
+ * until it is set, 1e12 at most. Returns the one before; a negative value only
+ * reads it. A limit that a call's waits reach ends that call early and sets
+ * the status above. */
 LCB200_API long long localCorrB200SetNormWaitLimit(long long nanoseconds);
 
 /* Library ABI version (major*10000 + minor*100 + patch). */

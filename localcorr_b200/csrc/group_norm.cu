@@ -628,7 +628,9 @@ bool feature_norm(const void* x, const void* dy, const void* weight, const void*
   p.act = act;
   p.slope = slope;
   p.eps = eps;
-  p.wait_ns = (uint64_t)wait_limit.load(std::memory_order_relaxed);
+  // the limit for each started GB: a CTA takes up to half a second for rows of a GB
+  p.wait_ns = (uint64_t)wait_limit.load(std::memory_order_relaxed) *
+              (1 + ((uint64_t)B * S * C * dtype_bytes(dtype) >> 30));
   p.slices = q.slices;
   p.slice_rows = q.slice_rows;
   p.fan = q.fan;
@@ -667,7 +669,7 @@ bool feature_norm(const void* x, const void* dy, const void* weight, const void*
 }
 
 long long feature_wait_limit(long long ns) {
-  return ns < 0 ? wait_limit.load() : wait_limit.exchange(ns);
+  return ns < 0 ? wait_limit.load() : wait_limit.exchange(std::min(ns, 1000000000000ll));
 }
 
 int feature_device_status(bool reset) {

@@ -242,3 +242,8 @@ def test_c_refuses_more_channels_than_the_kernels_count(lib):
         assert not _forward(lib, c=c, g=1) and "channels" in _lib.last_error(lib)
         assert lib.localCorrB200GroupNormWorkspaceBytes(1, 1, c, 1, _lib.F16, False) == 0
     assert not _forward(lib, c=2 ** 30, g=1) and "workspace" in _lib.last_error(lib)
+
+
+def test_c_wait_limit_is_bounded(lib):
+    before = lib.localCorrB200SetNormWaitLimit(2 ** 62)
+    assert lib.localCorrB200SetNormWaitLimit(before) == 10 ** 12
