@@ -9,6 +9,7 @@ import torch
 
 import localcorr_b200 as lc
 from localcorr_b200 import _lib, features
+from oracle import feature_maps as oracle
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -163,6 +164,123 @@ def test_equal_gradients_of_many_rows(shape, groups, dtype, value):
     got = _by_group(gx, groups).abs()
     assert bool((got <= tol * (1 + torch.finfo(dtype).eps)
                  + torch.finfo(dtype).smallest_normal).all())
+
+# ---------------------------------------------------------------------------
+# the forward's roundings, the parameters' gradients row by row, what dropout keeps
+# ---------------------------------------------------------------------------
+
+FORWARD = [((2, 46, 62, 256), 32), ((3, 47, 61, 96), 96), ((2, 3000, 33), 11), ((2, 37, 2048), 16),
+           ((5, 3, 3, 12), 4), ((1, 17, 4104), 8), ((1, 1, 256), 32)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("act", ["none", "relu", "silu", "leaky_relu"])
+@pytest.mark.parametrize("p", [0.0, 0.3])
+@pytest.mark.parametrize("shape,groups", FORWARD)
+def test_forward_to_its_roundings(shape, groups, p, act, dtype):
+    c = shape[-1]
+    x = (_randn(shape, 8) * (0.5 * _randn((c,), 9)).exp() + 3 * _randn((c,), 10)).to(dtype)
+    w = (1 + 0.3 * _randn((c,), 11)).float()
+    b = _randn((c,), 12).float()
+    y = lc.group_norm(x, groups, w, b, activation=act, negative_slope=0.1, p=p, rng=(3, 4))
+
+    mean, rstd = _statistics(x, groups, 1e-5)
+    mean, rstd = (t[:, None, :, None] for t in (mean, rstd))
+    grouped = _by_group(x, groups).shape
+    xhat = ((_by_group(x, groups) - mean) * rstd).reshape(shape)
+    shift = (mean.abs() * rstd).expand(grouped).reshape(shape)
+    z = xhat * w.double() + b.double()
+    e = 2.0 ** -24
+    # z = (x - mu) a + c: x - mu; 1/std and its product with the weight; c, which holds what
+    # mu loses in float32 (2^-24 of it); the sum
+    z_err = e * (3 * (xhat * w).abs() + b.abs() + e * shift * w.abs() + z.abs())
+    slope = 1.0
+    if act == "none":
+        want, err = z, 0.0
+    elif act == "relu":
+        want, err = z.clamp_min(0.0), 0.0
+    elif act == "leaky_relu":
+        slope32 = float(torch.tensor(0.1))
+        want = torch.where(z > 0, z, slope32 * z)
+        err = e * want.abs()
+    else:
+        # z sigma(z): exp within (2 + 1.173 |z|) ulp, which sigma takes on times 1 - sigma; the
+        # sum; a quotient within 2 ulp; the product. A ulp is 2^-23 at most
+        sigma = torch.sigmoid(z)
+        want, slope = z * sigma, 1.1
+        err = want.abs() * ((1 - sigma) * (2 + 1.173 * z.abs()) * 2 * e + e + 4 * e + e)
+    err = slope * z_err + err
+    if p > 0:
+        kept = lc.dropout(torch.ones_like(x, dtype=torch.float32), p, (3, 4)) != 0
+        t = int(p * 65536 + 0.5)
+        factor = 65536 / (65536 - t)  # and its rounding, and the product's
+        want, err = want * factor, err * factor + 2 * e * (want * factor).abs()
+        assert bool((y[~kept] == 0).all())
+        want, err = torch.where(kept, want, 0.0), torch.where(kept, err, 0.0)
+    u = torch.finfo(dtype).eps / 2
+    tol = (1 + 2 * u) * err + u * want.abs() + torch.finfo(dtype).smallest_normal * 2 * u
+    off = (y.double() - want).abs() - tol
+    assert bool((off <= 0).all()), float(off.max())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shape,groups", [((3, 2852, 64), 8), ((2, 8192, 128), 128),
+                                          ((2, 3000, 33), 11), ((5, 20, 48), 4),
+                                          ((1, 90, 4104), 8)])
+def test_gradients_of_single_rows(shape, groups, dtype):
+    # an output gradient of one row: what any row adds to the sums shows, and only that
+    b, rows, c = shape
+    x = _randn(shape, 13, torch.float32).to(dtype).requires_grad_(True)
+    w = (1 + 0.3 * _randn((c,), 14)).float().requires_grad_(True)
+    bias = torch.zeros(c, device=DEV, requires_grad=True)
+    y = lc.group_norm(x, groups, w, bias)
+    mean, rstd = _statistics(x.detach(), groups, 1e-5)
+    r = rstd[:, None, :, None]
+    v = (_by_group(x.detach(), groups) - mean[:, None, :, None]) * r  # xhat by group
+    e = 2.0 ** -24
+    u = torch.finfo(dtype).eps / 2
+    n = rows * (c // groups)
+    # ends of samples, of runs of rows a CTA has (whatever their length), and in between
+    for i, row in enumerate([0, 1, rows - 1] + [k * rows // 7 + k % 3 for k in range(1, 7)]):
+        sample, g = i % b, _randn((c,), 20 + i).to(dtype)
+        dy = torch.zeros_like(x)
+        dy[sample, row] = g
+        gx, gw, gb = torch.autograd.grad(y, (x, w, bias), dy, retain_graph=True)
+        assert torch.equal(gb, g.float())
+        xhat = v[sample, row].reshape(c)
+        want = g.double() * xhat
+        # x - mu, its product with dy, the result; mu's part below float32 is added in float64
+        assert bool(((gw.double() - want).abs() <= 4 * e * want.abs() + e * e * g.abs()).all())
+        wg = (w.detach().double() * g.double()).reshape(groups, -1)
+        vr = v[sample, row]
+        m1 = (wg.sum(1) / n)[None, :, None]
+        m2 = ((wg * vr).sum(1) / n)[None, :, None]
+        size1 = (wg.abs().sum(1) / n)[None, :, None]
+        size2 = ((wg * vr).abs().sum(1) / n)[None, :, None]
+        dz = torch.zeros_like(v[sample])
+        dz[row] = wg
+        want = r[sample] * (dz - m1 - v[sample] * m2)
+        # dx = a dz + (k2 (x - mu) + k3): the terms and two sums are rounded, a twice
+        tol = r[sample] * (4 * e * dz.abs() + 4 * e * size1 + 6 * e * v[sample].abs() * size2)
+        got = gx[sample].double().reshape(want.shape)
+        assert bool(((got - want).abs() <= tol + u * (want.abs() + tol) + 2.0 ** -140).all())
+        others = [k for k in range(b) if k != sample]
+        assert bool((gx[others] == 0).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("mode", ["element", "channel"])
+@pytest.mark.parametrize("shape", [(2, 31, 24), (2, 31, 33), (1, 7, 2056), (3, 1)])
+def test_dropout_drops_what_is_drawn_and_nothing_else(shape, mode, dtype):
+    # every value is far from 0: an element is 0 exactly where the draw says so
+    x = (_randn(shape, 15, torch.float32).sign() * 2 + 1).to(dtype)
+    f = oracle.drop_factors(shape, 0.4, 5, 6, mode == "channel").expand(shape)
+    y = lc.dropout(x, 0.4, (5, 6), mode=mode).cpu()
+    assert torch.equal(y == 0, f == 0)
+    r = torch.full_like(x, 0.5)
+    z = lc.dropout(x, 0.4, (5, 6), residual=r, mode=mode).cpu()
+    assert torch.equal(z == 0.5, f == 0)
+
 
 # ---------------------------------------------------------------------------
 # what autograd is told
