@@ -9,7 +9,7 @@
 
 namespace lcb200 {
 
-bool stream_norm(const NormArgs& p, int dtype, bool backward, cudaStream_t s);
+Streamed stream_norm(const NormArgs& p, int dtype, bool backward, cudaStream_t s);
 int stream_norm_status(bool reset);
 int stream_ctas();  // resident CTAs
 int stream_stage_rows(int C, int dtype, bool backward);  // rows of a stage, at least 1
@@ -523,6 +523,8 @@ Plan make_plan(int B, long long S, int C, int dtype, bool backward) {
   return q;
 }
 
+// Streamed maps have the plain kernels' rows too: a context may have no room for all CTAs of
+// the streamed ones at once.
 struct Layout {  // byte offsets
   size_t flags, part, set_part, bpart, sums, coef, total;
 };
@@ -643,7 +645,7 @@ bool feature_norm(const void* x, const void* dy, const void* weight, const void*
   p.chunk = q.chunk;
   p.chunks = q.chunks;
   p.tickets = out ? 2 * q.units : q.units;
-  const bool stream = !q.samples && streams(C, G, dtype, vec_width(dtype, C, x, out, dy));
+  bool stream = !q.samples && streams(C, G, dtype, vec_width(dtype, C, x, out, dy));
   p.ticket = reinterpret_cast<uint32_t*>(w);
   p.done = p.ticket + 2;
   p.sets_done = p.done + (size_t)B * q.sets;
@@ -656,12 +658,19 @@ bool feature_norm(const void* x, const void* dy, const void* weight, const void*
   p.dweight = dweight;
   p.dbias = dbias;
   p.drop = drop;
-  if (!q.samples &&
-      (stream ? cudaMemsetAsync(w + l.part, 0xff, sizeof(double2) * (size_t)G * q.slots, s)
-              : cudaMemsetAsync(w, 0, l.flags, s)) != cudaSuccess)
-    return check_launch("group norm: memset of the counters");
-  if (!stream) return launch(p, dtype, backward, q.samples, s);
-  if (!stream_norm(p, dtype, backward, s)) return false;
+  if (stream) {
+    if (cudaMemsetAsync(w + l.part, 0xff, sizeof(double2) * (size_t)G * q.slots, s) !=
+        cudaSuccess)
+      return check_launch("group norm: memset of the entries");
+    const Streamed done = stream_norm(p, dtype, backward, s);
+    if (done == Streamed::kFailed) return false;
+    stream = done == Streamed::kDone;  // else the plain kernels, which need no co-residency
+  }
+  if (!stream) {
+    if (!q.samples && cudaMemsetAsync(w, 0, l.flags, s) != cudaSuccess)
+      return check_launch("group norm: memset of the counters");
+    return launch(p, dtype, backward, q.samples, s);
+  }
   if (!backward) return true;
   if (dtype == LCB200_F32) return launch_params<float>(p, p.ctas * p.teams, s);
   if (dtype == LCB200_F16) return launch_params<__half>(p, p.ctas * p.teams, s);

@@ -88,6 +88,10 @@ struct NormArgs {
   DropArgs drop;
 };
 
+// What came of a launch of the streamed kernels. kNoRoom: their CTAs do not fit the context
+// all at once (one that has a part of the GPU's multiprocessors), nothing was launched.
+enum class Streamed { kDone, kFailed, kNoRoom };
+
 // Runs of a chunk of the streamed kernels: one a CTA, fewer where that would leave less
 // than a stage.
 __host__ __device__ inline int chunk_parts(long long rows, int stage_rows, int ctas) {

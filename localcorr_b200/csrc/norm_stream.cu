@@ -919,20 +919,24 @@ __global__ void __launch_bounds__(kBlock, kPerSm) norm_backward_stream(NormArgs 
 
 // ---- host ----------------------------------------------------------------------------
 template <typename K>
-bool launch_kernel(K kernel, size_t smem, const NormArgs& p, const char* what, cudaStream_t s) {
+Streamed launch_kernel(K kernel, size_t smem, const NormArgs& p, const char* what,
+                       cudaStream_t s) {
   // the static shared memory counts towards the 48 KB that need no opt-in
-  if (!ensure_smem_attr((const void*)kernel, smem + 1024)) return false;
+  if (!ensure_smem_attr((const void*)kernel, smem + 1024)) return Streamed::kFailed;
   NormArgs args = p;
   void* argv[] = {&args};
-  if (cudaLaunchCooperativeKernel((const void*)kernel, dim3(p.ctas * p.teams), dim3(kBlock), argv, smem,
-                                  s) != cudaSuccess)
-    return check_launch(what);
-  count_launch();
-  return check_launch(what);
+  const cudaError_t e = cudaLaunchCooperativeKernel((const void*)kernel, dim3(p.ctas * p.teams),
+                                                    dim3(kBlock), argv, smem, s);
+  if (e == cudaErrorCooperativeLaunchTooLarge) {
+    cudaGetLastError();
+    return Streamed::kNoRoom;
+  }
+  if (e == cudaSuccess) count_launch();
+  return check_launch(what) ? Streamed::kDone : Streamed::kFailed;
 }
 
 template <typename T, bool WHOLE, bool DROP>
-bool launch_w(const NormArgs& p, bool backward, cudaStream_t s) {
+Streamed launch_w(const NormArgs& p, bool backward, cudaStream_t s) {
   if (!backward)
     return launch_kernel(norm_forward_stream<T, WHOLE, DROP>,
                          sizeof(ForwardShared<T, WHOLE>) + sizeof(double2) * p.G, p, "group norm",
@@ -946,7 +950,7 @@ bool launch_w(const NormArgs& p, bool backward, cudaStream_t s) {
 }
 
 template <typename T>
-bool launch_t(const NormArgs& p, bool backward, cudaStream_t s) {
+Streamed launch_t(const NormArgs& p, bool backward, cudaStream_t s) {
   const bool drop = p.drop.threshold != 0;
   if (p.Cg % (16 / sizeof(T)) == 0)
     return drop ? launch_w<T, true, true>(p, backward, s) : launch_w<T, true, false>(p, backward, s);
@@ -955,7 +959,7 @@ bool launch_t(const NormArgs& p, bool backward, cudaStream_t s) {
 
 }  // namespace
 
-bool stream_norm(const NormArgs& p, int dtype, bool backward, cudaStream_t s) {
+Streamed stream_norm(const NormArgs& p, int dtype, bool backward, cudaStream_t s) {
   if (dtype == LCB200_F32) return launch_t<float>(p, backward, s);
   if (dtype == LCB200_F16) return launch_t<__half>(p, backward, s);
   return launch_t<__nv_bfloat16>(p, backward, s);

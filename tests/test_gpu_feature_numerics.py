@@ -344,3 +344,37 @@ def test_hooks_see_all_that_is_saved():
         torch.autograd.grad(y.sum(), x)
         with pytest.raises(RuntimeError, match="second time"):
             torch.autograd.grad(y.sum(), x)
+
+
+@pytest.mark.parametrize("shape,groups,dtype", [((3, 4000, 64), 8, torch.float16),
+                                                ((2, 2000, 64), 64, torch.float32)])
+def test_context_with_a_part_of_the_multiprocessors(shape, groups, dtype):
+    # the streamed kernels' CTAs do not fit all at once: the plain kernels take the call
+    green = pytest.importorskip("torch.cuda.green_contexts")
+    if not green.SUPPORTED:
+        pytest.skip("green contexts not supported")
+    x, dy = (_randn(shape, 30 + i, torch.float32).to(dtype) for i in range(2))
+    w = torch.linspace(0.5, 1.5, shape[-1], device=DEV)
+
+    def call():
+        y, stats, _ = features.group_norm_forward(x, w, None, groups, 1e-5, "silu", 0.0, 0.0, False,
+                                                  None, 0, 0)
+        return y, *features.group_norm_backward(dy, x, w, None, stats, None, groups, "silu", 0.0,
+                                                0.0, False)[:2]
+
+    want = call()
+    torch.cuda.synchronize()
+    context = green.GreenContext.create(num_sms=16, device_id=torch.cuda.current_device())
+    context.set_context()
+    try:
+        got = call()
+        torch.cuda.synchronize()
+    finally:
+        context.pop_context()
+    # float32 roundings of two orders of summation, 2^-18 at most, then the rounding of either
+    u = torch.finfo(dtype).eps / 2
+    for a, b in zip(got, want):
+        e = u if a.dtype == dtype else 2.0 ** -24
+        scale = b.double().abs().max()
+        assert bool(((a.double() - b.double()).abs()
+                     <= 2 * e * b.double().abs() + 2.0 ** -18 * scale).all())
