@@ -315,7 +315,8 @@ LCB200_API bool launchLocalCorrB200PyramidBackwardFmap2Pull(
  * long longs at `rng` (device; a captured graph can advance them between
  * replays) or, with rng NULL, the arguments seed and offset. rng_used (device,
  * two long longs, may be NULL) receives the stream that was used; pass it as
- * `rng` of the backward. */
+ * `rng` of the backward. Calls on empty maps succeed and write nothing (the
+ * group norm's backward: zeros to grad_weight and grad_bias). */
 
 /* y = residual + dropout(x); residual may be NULL. The gradient of x is the
  * same call on the output gradient without a residual (the residual's

@@ -164,6 +164,12 @@ def _ptr(t):
     return t.data_ptr() if t is not None else None
 
 
+def _by_product(x, shape, dtype):
+    """What a launch writes beside its map; an empty map's call writes nothing."""
+    make = torch.empty if x.numel() else torch.zeros
+    return make(shape, dtype=dtype, device=x.device)
+
+
 def dropout_forward(x, residual, p, channel, rng, seed, offset):
     """(residual + dropout(x), the stream used [2]) of contiguous-or-copied maps."""
     lib = _lib.require_library()
@@ -174,7 +180,7 @@ def dropout_forward(x, residual, p, channel, rng, seed, offset):
         rng = rng.contiguous()
     b, rows, c = _rows(x)
     y = torch.empty_like(x)
-    used = torch.empty(2, dtype=torch.int64, device=x.device)
+    used = _by_product(x, 2, torch.int64)
     dev = x.get_device()
     with _on_device(dev):
         ok = _timed("dropout", lambda: lib.launchLocalCorrB200Dropout(
@@ -228,8 +234,8 @@ def group_norm_forward(x, weight, bias, num_groups, eps, activation, negative_sl
         rng = rng.contiguous()
     b, rows, c = _rows(x)
     y = torch.empty_like(x)
-    stats = torch.empty((b, num_groups, 2), dtype=torch.float64, device=x.device)
-    used = torch.empty(2, dtype=torch.int64, device=x.device) if p > 0 else None
+    stats = _by_product(x, (b, num_groups, 2), torch.float64)
+    used = _by_product(x, 2, torch.int64) if p > 0 else None
     ws = _norm_workspace(x, b, rows, c, num_groups, False)
     dev = x.get_device()
     with _on_device(dev):

@@ -378,3 +378,12 @@ def test_context_with_a_part_of_the_multiprocessors(shape, groups, dtype):
         scale = b.double().abs().max()
         assert bool(((a.double() - b.double()).abs()
                      <= 2 * e * b.double().abs() + 2.0 ** -18 * scale).all())
+
+
+def test_by_products_of_empty_maps_are_zero():
+    torch.full((4096,), 7.0, dtype=torch.float64, device=DEV)  # what freed memory may hold
+    x = torch.zeros(3, 0, 8, device=DEV)
+    y, stats, used = torch.ops.localcorr.group_norm(x, None, None, 2, 1e-5, "none", 0.0, 0.5,
+                                                    False, None, 1, 2)
+    assert y.shape == x.shape and bool((stats == 0).all()) and bool((used == 0).all())
+    assert bool((torch.ops.localcorr.dropout(x, None, 0.5, False, None, 1, 2)[1] == 0).all())
