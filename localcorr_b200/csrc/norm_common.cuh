@@ -13,12 +13,18 @@
 // needed before the first output, so a sample is read twice; see the launchers
 // for how the second read comes out of L2.
 //
-// Numerics. The sums are of x - K and (x - K)^2 with K the group's first value, float64
-// from the first addition on. K is one of the group's n values, so (mu - K)^2 is at most
-// (n - 1) var, and a few var for a map like any other, however far its mean lies from 0:
-// the cancellation in var = E[(x - K)^2] - (mu - K)^2 costs that factor of 2^-53 and no
-// more, and a constant group's var is 0 exactly. (Sums of x and x^2 left 1/std 3e-7 off
-// at mean / std = 1e5, 1e-4 off at 1e6. Float32 sums of (x - K)^2 over 110 rows left it
+// Numerics. The sums are of d = x - K and d^2, float64 from the first addition on, and
+// var = (n sum d^2 - (sum d)^2) / n^2 with split products: it may cancel to (mu - K)^2 / var
+// of what the sums lost to rounding.
+//   float32 maps: K is the group's first value. As one of the n values it has (mu - K)^2 <=
+// (n - 1) var, and a few var in a map like any other, however far its mean lies from 0.
+//   16-bit maps: K = 0. Where mu^2 / var is large nearly all values lie in one binade: they are
+// whole multiples, of 8 or 11 bits, of one step, so their sums and those of their squares (22
+// bits and log2 n) are exact; each other value costs a rounding, but has a share of var. (K
+// here would be a third float64 operation an element, 4 % of instance norm's forward, and the
+// registers of rows wider than a CTA: 248 us instead of 199 for 8 x 6400 x 2304.)
+// A constant group's var is 0 exactly. (Plain E[x^2] - mu^2 left 1/std of float32 maps 1e-6
+// off at mean / std = 1e5, 1e-4 off at 1e6. Float32 sums of d^2 over 110 rows left it
 // 1.7e-7 off for bfloat16 maps: squares of odd integers are 1 modulo 8, so their roundings
 // do not average out.) That matters because a rectifier's gradient jumps at z = 0: with
 // 1.7e-7, one training step in three of a 67 million element map had elements on the wrong
@@ -78,7 +84,7 @@ struct NormArgs {
   uint32_t* sets_done;  // [B] finished sets
   uint32_t* ready;      // [B] 1: statistics (backward: coef) are there
   // (the plain kernels' rows; the others have a row per slot or CTA)
-  double2* part;        // forward: [B, slices, G] (sum x - K, sum (x - K)^2); streamed: [slots, G]
+  double2* part;        // forward: [B, slices, G] (sum d, sum d^2); streamed: [slots, G]
   float2* bpart;        // backward: [B, slices, C] (sum dz, sum dz (x - mu))
   double2* set_part;    // [B, sets, G (backward: C)] sums of a set's slices
   double2* sums;        // backward: [B, C] (A, X); otherwise a CTA's sum of them, [CTAs, C]
@@ -190,20 +196,21 @@ __device__ __forceinline__ float affine_z(const Affine& f, float x) {
 }
 
 // ---- the end of a sample: statistics, or coefficients of dx --------------------
-// The value K that a group's sums are centred on: its first.
+// The value K that a group's sums are centred on.
 template <typename T>
 __device__ __forceinline__ double group_shift(const NormArgs& p, int b, int g) {
+  if (sizeof(T) < 4) return 0.0;
   return (double)ldf(reinterpret_cast<const T*>(p.x) + (long long)b * p.S * p.C +
                      (long long)g * p.Cg);
 }
 
-// One group's mean and 1/std from its (sum x - K, sum (x - K)^2).
+// One group's mean and 1/std from its (sum d, sum d^2).
 __device__ __forceinline__ double2 finish_stats(const NormArgs& p, double2 v, double shift) {
-  const double inv = 1.0 / ((double)p.S * p.Cg);
-  const double mean = v.x * inv;
-  double var = v.y * inv - mean * mean;
+  const double n = (double)p.S * p.Cg, inv = 1.0 / n;
+  const double nq = n * v.y, ss = v.x * v.x;
+  double var = ((nq - ss) + (fma(n, v.y, -nq) - fma(v.x, v.x, -ss))) * inv * inv;
   var = var < 0.0 ? 0.0 : var;  // rounding below zero; NaN stays
-  return make_double2(shift + mean, 1.0 / sqrt(var + p.eps));
+  return make_double2(fma(v.x, inv, shift), 1.0 / sqrt(var + p.eps));
 }
 
 // True in every thread of the CTA that finished last of `count` at *counter;

@@ -465,7 +465,7 @@ template <typename T, bool WHOLE>
 struct ForwardShared {
   static constexpr int kV = 16 / sizeof(T), kStages = WHOLE ? 5 : 4;
   RingShared<1, kStages> ring;
-  double2 sums[kS * (WHOLE ? 1 : kV)];  // (sum x - K, sum (x - K)^2) of each thread
+  double2 sums[kS * (WHOLE ? 1 : kV)];  // (sum d, sum d^2) of each thread
   double2 stats[1];                     // [G] of the second pass's sample
 };
 
@@ -531,7 +531,7 @@ __device__ __forceinline__ bool apply_unit(const NormArgs& p, const Place& at, C
   constexpr int V = 16 / sizeof(T), N = WHOLE ? 1 : V / 2;
   const int b = in.sample(), c0 = at.col * V;
   const bool top = in.now & kTop;
-  // on their way while the sums are: sample_sums starts with a barrier
+  // K, on its way while the sums are: sample_sums starts with a barrier
   for (int g = threadIdx.x; g < p.G; g += kS) stats[g].x = group_shift<T>(p, b, g);
   sample_sums(p, b, &in.r.abort, red, [&](int g, double2 t) {
     stats[g] = finish_stats(p, t, stats[g].x);

@@ -102,6 +102,38 @@ def test_small_variance_far_from_zero_without_eps(shape, groups):
     assert bool((off <= 0).all())
 
 
+@pytest.mark.parametrize("eps", [1e-5, 0.0])
+@pytest.mark.parametrize("dtype,mean,std", [
+    (torch.float16, 1000.0, 1.0), (torch.float16, 30000.0, 20.0), (torch.float16, -2048.0, 0.6),
+    (torch.float16, 0.01, 1e-4), (torch.bfloat16, 300.0, 1.0), (torch.bfloat16, 1e4, 40.0),
+    (torch.bfloat16, -3e4, 1000.0), (torch.bfloat16, 1e18, 1e17)])
+@pytest.mark.parametrize("shape,groups", SIZES)
+def test_statistics_of_16_bit_maps_far_from_zero(shape, groups, dtype, mean, std, eps):
+    x = (_randn(shape, 16) * std + mean).to(dtype)
+    want_mean, want_rstd = _statistics(x, groups, eps)
+    got_mean, got_rstd = _kernel_statistics(x, groups, eps)
+    # nearly all values lie in two binades: their sums are exact. What is rounded (2^13 sums at
+    # most) is weighed with 1 + mean^2 / var, which rounding to the type keeps below 2^22
+    assert bool(want_rstd.isfinite().all())
+    torch.testing.assert_close(got_rstd, want_rstd, rtol=2.0 ** -36, atol=0)
+    torch.testing.assert_close(got_mean, want_mean, rtol=2.0 ** -45, atol=0)
+
+
+@pytest.mark.parametrize("shape,groups", SIZES)
+@pytest.mark.parametrize("dtype,level", [(torch.float16, 1000.0), (torch.bfloat16, 1000.0)])
+def test_small_variance_of_16_bit_maps_without_eps(shape, groups, dtype, level):
+    # one value in a hundred is a step above the others, one in a thousand is 0
+    x = torch.full(shape, level, dtype=dtype, device=DEV)
+    x.view(-1)[::97] = level + (0.5 if dtype == torch.float16 else 4.0)
+    x.view(-1)[::997] = 0.0
+    want_mean, want_rstd = _statistics(x, groups, 0.0)
+    got_mean, got_rstd = _kernel_statistics(x, groups, 0.0)
+    # multiples of one step throughout: exact sums, a few roundings behind them
+    assert bool(want_rstd.isfinite().all())
+    torch.testing.assert_close(got_rstd, want_rstd, rtol=2.0 ** -45, atol=0)
+    torch.testing.assert_close(got_mean, want_mean, rtol=2.0 ** -48, atol=0)
+
+
 @pytest.mark.parametrize("shape,groups", SIZES)
 def test_constant_groups_give_the_bias(shape, groups):
     x = torch.full(shape, 1234567.0, device=DEV)
