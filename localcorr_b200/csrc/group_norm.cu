@@ -1,8 +1,10 @@
 // Group norm: plan and launch, the kernels for whole samples, and the plain kernels for
 // maps that the streamed ones (norm_stream.cu) do not take: rows that are no whole
 // number of aligned 16-byte vectors, too wide, or of too many groups. The plain kernels
-// move 1 to 2.5 TB/s where the streamed ones move 3 to 4 (8 x 32400 x 99 float16
-// element by element: 92 us forward; x 96: 35 us).
+// move 0.6 to 2.4 TB/s where the streamed ones move 2.7 to 4.2: 8 x 32400 x 99 float16, element
+// by element, takes 97 us forward and 211 backward, x 96 takes 32 and 54; 8 x 6400 x 2304,
+// wider than a CTA, takes 200 and 1105 (each slice of 16 rows writes and reads again a pair
+// of sums for every channel).
 #include <atomic>
 
 #include "norm_common.cuh"

@@ -130,7 +130,9 @@ __device__ __forceinline__ void put_param(void* p, int f32, int c, double v) {
   else stf(reinterpret_cast<T*>(p) + c, (float)v);
 }
 
-// sigma(z); exp(-z) overflowing to infinity gives 0.
+// sigma(z) by the fast exponential (2 + 1.173 |z| ulp) and quotient (2 ulp): their error counts
+// times 1 - sigma, so z sigma(z) is within 6 ulp for z > -1 and within 5 + 1.2 |z| ulp of its
+// shrinking value below. exp(-z) overflowing to infinity gives 0.
 __device__ __forceinline__ float sigmoid(float z) { return __fdividef(1.f, 1.f + __expf(-z)); }
 
 __device__ __forceinline__ float act_value(float z, int act, float slope) {
