@@ -344,8 +344,9 @@ def group_norm(x, num_groups, weight=None, bias=None, eps=1e-5, activation="none
     ([C], either may be None; float32 or x's dtype, both the same). ``activation`` is "none", "relu",
     "silu" or "leaky_relu" (with ``negative_slope``). With ``p`` > 0 the result
     is dropped out as :func:`dropout` does with ``rng`` and ``dropout_mode``.
-    Statistics are float64, the result is rounded to x's dtype once; results
-    repeat bit for bit. A group of a single value gives ``bias``. Inputs that
+    Statistics are float64, also of maps far from zero; the result is rounded to
+    x's dtype once; results repeat bit for bit for equal sizes and alignment. A
+    group of equal values gives ``bias`` (NaN with ``eps`` = 0). Inputs that
     are not contiguous are copied. Gradients for x, weight and bias (once
     differentiable).
     """
